@@ -242,6 +242,88 @@ B200Q8_API int b200q8_rms_norm(void* out, const void* x, int dtype, const float*
 B200Q8_API int b200q8_silu_mul(void* out, const void* gate_up, int dtype, size_t M, size_t K,
                                b200q8_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * 4-bit weights with a scale per group.  No vvllm counterpart (the reference
+ * quantizes to 8 bits only); for models whose decode step is bound by the
+ * weights' bytes, at half the bytes of the int8 path.
+ *
+ * Format: w[n, k] = q[n, k] * s[n, k / group], q in -8..7, s a bfloat16.
+ *   q4     uint8 [N, ceil(K / 2)]: byte j of a row holds element 2j in its low and 2j + 1 in its
+ *          high four bits, as q + 8; the last high half of an odd row is 8 (the value 0).
+ *   scales uint16 (bfloat16 bits) [N, ceil(K / group)]; a row's last group may be short.
+ *   group  32, 64 or 128.
+ * Rows are independent, so a row range of both arrays is the shard of those output channels.
+ * ------------------------------------------------------------------------ */
+
+/* q4, scales = 4-bit group quantization of w [N, K] (fp32): per group s = the bfloat16 nearest to
+ * max |w| / 7 (NaN skipped), q = w / s rounded to the nearest integer, ties to even, within -8..7.
+ * Groups whose s is 0 and NaN weights get q = 0; a group that holds an infinity gets s = +inf (and
+ * its products are NaN).  w must not overlap the outputs. */
+B200Q8_API int b200q8_quantize_q4(const float* w, size_t N, size_t K, int group, uint8_t* q4, uint16_t* scales,
+                                  b200q8_stream_t stream);
+/* The same from bfloat16 bits. */
+B200Q8_API int b200q8_quantize_q4_bf16(const uint16_t* w, size_t N, size_t K, int group, uint8_t* q4, uint16_t* scales,
+                                       b200q8_stream_t stream);
+
+/* out [R, K] (fp32: exact; fp16: rounded once) = the values of the rows rows[0..R) (device int32;
+ * the token lookup of a tied 4-bit embedding; the same row may come more than once), or with rows
+ * NULL of all rows (then R must be N).  An index outside [0, N) gives a row of zeros. */
+B200Q8_API int b200q8_dequantize_q4(void* out, int out_dtype, const uint8_t* q4, const uint16_t* scales, int group,
+                                    const int32_t* rows, size_t R, size_t N, size_t K, b200q8_stream_t stream);
+
+/* out[M, N] = inp[M, K] . w[N, K]^T + bias[N]; bias may be NULL.  inp and out are fp32 or fp16;
+ * products are exact and sums fp32, whatever the types.  inp must not overlap out. */
+B200Q8_API int b200q8_linear_q4(void* out, int out_dtype, const void* inp, int in_dtype, const uint8_t* q4,
+                                const uint16_t* scales, int group, const float* bias, size_t M, size_t N, size_t K,
+                                b200q8_stream_t stream);
+/* The same plus residual[M, N] (out_dtype), added last; residual may be out itself, or NULL. */
+B200Q8_API int b200q8_linear_q4_add(void* out, int out_dtype, const void* inp, int in_dtype, const uint8_t* q4,
+                                    const uint16_t* scales, int group, const float* bias, const void* residual,
+                                    size_t M, size_t N, size_t K, b200q8_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * The step between the lm_head's logits and the token.  vvllm has temperature and top-p only
+ * (src/sampler/sampler.cc); servers also penalize repeated tokens, bias listed tokens and mask what
+ * a grammar does not allow.
+ * ------------------------------------------------------------------------ */
+
+/* What process_logits applies; zero-initialize, then set what is wanted.  All pointers are device
+ * pointers with one row (or value) per logits row; strides are in elements, and 0 shares one row
+ * among all. */
+typedef struct b200q8_logit_rules {
+    const int32_t* history;      /* tokens of the row so far: prompt, then output; NULL: no penalties */
+    size_t history_stride;
+    size_t history_count;        /* entries a history row has room for */
+    const int32_t* history_len;  /* [M] live tokens of each history row (needed with history) */
+    const int32_t* prompt_len;   /* [M] how many of them are prompt; NULL: none */
+    const float* repetition;     /* [M] or NULL (1); the penalties act on the history's tokens only */
+    const float* presence;       /* [M] or NULL (0) */
+    const float* frequency;      /* [M] or NULL (0) */
+    const int32_t* bias_ids;     /* tokens with a bias; NULL: none */
+    const float* bias_values;    /* their biases, laid out like bias_ids */
+    size_t bias_stride;
+    size_t bias_count;           /* entries of a row */
+    const int32_t* bias_len;     /* [M] live entries of each row; NULL: bias_count */
+    const uint32_t* allowed;     /* bit i % 32 of word i / 32: token i may be chosen; NULL: all may */
+    size_t allowed_stride;
+} b200q8_logit_rules;
+
+/* Per row m and token i < V, in fp32, each operation rounded once:
+ *   v = logits[m, i]
+ *   i anywhere in the history:            v = v > 0 ? v / repetition : v * repetition
+ *   i c > 0 times behind the prompt:      v = v - frequency * c, then v = v - presence
+ *   i in the bias list:                   v = v + bias (a token listed twice takes its last entry)
+ *   i not allowed:                        v = -inf, whatever it was
+ *   out[m, i] = v in out_dtype;  argmax[m] = the first largest out[m, i] among the allowed i, in the
+ *   order of b200q8_linear_q8_argmax (a NaN wins only as the first allowed token); -1 if none is allowed.
+ * out may be NULL (only the tokens are wanted), or logits itself (same type and stride); it must not
+ * overlap logits otherwise.  argmax (int32 [M]) may be NULL.  rules may be NULL.  Token ids outside
+ * [0, V) in the lists are ignored; lengths are clamped to [0, history_count] and [0, bias_count].
+ * One launch, no scratch. */
+B200Q8_API int b200q8_process_logits(void* out, int out_dtype, size_t out_stride, const void* logits, int in_dtype,
+                                     size_t in_stride, size_t M, size_t V, const b200q8_logit_rules* rules,
+                                     int32_t* argmax, b200q8_stream_t stream);
+
 /* Device error word of the current device: bit 0 is set when a bounded wait
  * inside a tensor-core kernel gave up; bit 1 when a sharded call's wait for
  * the peers' outputs ran out (2 s).  Either way the outputs are invalid.

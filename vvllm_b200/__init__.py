@@ -35,6 +35,12 @@ from ._lib import (  # noqa: F401
     ST_F32,
     ST_I8,
     ST_OTHER,
+    dequantize_q4,
+    linear_q4,
+    linear_q4_add,
+    process_logits,
+    quantize_q4,
+    quantize_q4_bf16,
     rms_norm,
     rms_norm_linear_q8,
     linear_q8_group,

@@ -330,6 +330,17 @@ int linear_impl(void* out, int out_dtype, const void* inp, int in_dtype, const i
 }
 
 }  // namespace
+
+int current_device(int* num_sms, size_t* max_smem)
+{
+    DeviceInfo d;
+    const int st = device_info(&d);
+    if (st) return st;
+    *num_sms = d.num_sms;
+    *max_smem = d.max_smem;
+    return B200Q8_OK;
+}
+
 }  // namespace b200q8
 
 using namespace b200q8;

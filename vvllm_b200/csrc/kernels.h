@@ -152,6 +152,49 @@ cudaError_t launch_q8_gemm_tc(const LinearArgs& a, int num_sms, const TcScratch&
 bool gemm_tc_supports(const LinearArgs& a);
 void gemm_tc_scratch_need(const LinearArgs& a, int num_sms, size_t* ws_floats, size_t* counters);
 
+// 4-bit group quantization (format: q4_common.cuh): q4 [N, ceil(K/2)], scales (bf16 bits)
+// [N, ceil(K/group)] from w [N, K] fp32 or bf16 bits; group is 32, 64 or 128.
+cudaError_t launch_q4_quantize(const void* w, int w_bf16, size_t N, size_t K, int group, uint8_t* q4, uint16_t* scales,
+                               int num_sms, cudaStream_t stream);
+// out [R, K]: the values of rows rows[0..R) (an index outside [0, N): zeros), or of all N = R rows (rows null).
+cudaError_t launch_q4_dequantize(void* out, int out_dtype, const uint8_t* q4, const uint16_t* scales, int group,
+                                 const int* rows, size_t R, size_t N, size_t K, int num_sms, cudaStream_t stream);
+
+struct Q4Args {
+    const void* x = nullptr;           // [M, K] activations (in_dtype)
+    const uint8_t* q4 = nullptr;       // [N, ceil(K/2)] codes
+    const uint16_t* scales = nullptr;  // [N, ceil(K/group)] bf16 bits
+    const float* bias = nullptr;       // [N] or null
+    const void* res = nullptr;         // [M, N] residual (out_dtype) or null
+    void* out = nullptr;               // [M, N] (out_dtype)
+    size_t M = 0, N = 0, K = 0;
+    int group = 0, in_dtype = kF32, out_dtype = kF32;
+};
+// Any shape and alignment.
+cudaError_t launch_q4_linear_generic(const Q4Args& a, cudaStream_t stream);
+
+struct LogitArgs {
+    void* out = nullptr;            // [M, V] rows of out_stride elements, or null
+    const void* logits = nullptr;   // [M, V] rows of in_stride elements; may be out
+    int* argmax = nullptr;          // [M] or null
+    size_t M = 0, V = 0, in_stride = 0, out_stride = 0;
+    int in_dtype = kF32, out_dtype = kF32;
+    const int* history = nullptr;      // rows of history_count tokens, the first history_len[m] of them live
+    const int* history_len = nullptr;  // [M]
+    const int* prompt_len = nullptr;   // [M] or null (0)
+    size_t history_stride = 0, history_count = 0;
+    const float* repetition = nullptr;  // [M] or null (1)
+    const float* presence = nullptr;    // [M] or null (0)
+    const float* frequency = nullptr;   // [M] or null (0)
+    const int* bias_ids = nullptr;      // rows of bias_count tokens, the first bias_len[m] of them live
+    const float* bias_values = nullptr; // the same rows
+    const int* bias_len = nullptr;      // [M] or null (bias_count)
+    size_t bias_stride = 0, bias_count = 0;
+    const uint32_t* allowed = nullptr;  // [M] rows of allowed_stride words, bit i % 32 of word i / 32; or null
+    size_t allowed_stride = 0;
+};
+cudaError_t launch_logits(const LogitArgs& a, size_t max_smem, cudaStream_t stream);
+
 // Reads (and optionally clears) the device error word the tensor-core kernel
 // sets when a bounded wait gives up (bit 0).
 cudaError_t read_kernel_error(int* code, bool clear);
@@ -165,6 +208,9 @@ cudaError_t launch_gather_permute(const void* src, void* dst, int elem_bytes, si
 // aligned.  Same arithmetic as the prologue fused into the SIMT GEMV and the digit GEMV's prep.
 cudaError_t launch_prologue(int pro, const void* x, void* out, int dtype, const float* norm_w, float eps, size_t M,
                             size_t K, bool pdl, cudaStream_t stream);
+
+// SM count and opt-in shared memory of the current device, as a status (B200Q8_ERR_UNSUPPORTED: not sm_100).
+int current_device(int* num_sms, size_t* max_smem);
 
 // Error reporting of the C ABI: record the message b200q8_last_error() returns, return status.
 int fail(int status, const char* fmt, ...);
