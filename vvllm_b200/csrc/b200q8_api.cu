@@ -331,6 +331,15 @@ int linear_impl(void* out, int out_dtype, const void* inp, int in_dtype, const i
 
 }  // namespace
 
+int stream_scratch(size_t ws_floats, size_t counters, size_t act_bytes, int num_sms, cudaStream_t stream, TcScratch* out)
+{
+    ScratchNeed need;
+    need.ws = ws_floats;
+    need.counters = counters;
+    need.act = act_bytes;
+    return get_scratch(need, num_sms, stream, out);
+}
+
 int current_device(int* num_sms, size_t* max_smem)
 {
     DeviceInfo d;
@@ -417,11 +426,12 @@ int b200q8_linear_q8_ex(void* out, int out_dtype, const void* inp, int in_dtype,
 int b200q8_kernel_error(int* code, int clear)
 {
     if (!code) return fail(B200Q8_ERR_INVALID, "kernel_error: null code");
-    int c1 = 0, c2 = 0;
+    int c1 = 0, c2 = 0, c3 = 0;
     cudaError_t e = read_kernel_error(&c1, clear != 0);
     if (e == cudaSuccess) e = read_kernel_error_i8(&c2, clear != 0);
+    if (e == cudaSuccess) e = read_kernel_error_q4(&c3, clear != 0);
     if (e != cudaSuccess) return cuda_fail(e, "kernel_error: read device word");
-    *code = c1 | c2;
+    *code = c1 | c2 | c3;
     if (clear && *code) {
         int dev = 0;
         if ((e = cudaGetDevice(&dev)) != cudaSuccess) return cuda_fail(e, "cudaGetDevice");

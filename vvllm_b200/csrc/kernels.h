@@ -172,6 +172,19 @@ struct Q4Args {
 };
 // Any shape and alignment.
 cudaError_t launch_q4_linear_generic(const Q4Args& a, cudaStream_t stream);
+// Streaming tensor-core kernel: K % 32 == 0, q4 and x 16-byte, scales 4-byte aligned.  Any M, in groups of
+// up to 32 (fp16) or 10 (fp32) tokens.  cudaErrorNotSupported: alignment, or K beyond its shared memory.
+bool q4_stream_supports(const Q4Args& a);
+cudaError_t launch_q4_stream(const Q4Args& a, int num_sms, size_t max_smem, cudaStream_t stream);
+
+// The error word of that kernel's bounded waits (bit 0).
+cudaError_t read_kernel_error_q4(int* code, bool clear);
+
+// The tcgen05 GEMM on 4-bit weights: fp16 activations, K % 32 == 0, aligned pointers, any M.  act_bytes holds
+// the scales as its dequantizers read them (written by a kernel before it in each call).
+bool q4_gemm_tc_supports(const Q4Args& a);
+void q4_gemm_tc_scratch_need(const Q4Args& a, int num_sms, size_t* ws_floats, size_t* counters, size_t* act_bytes);
+cudaError_t launch_q4_gemm_tc(const Q4Args& a, int num_sms, const TcScratch& scratch, cudaStream_t stream);
 
 struct LogitArgs {
     void* out = nullptr;            // [M, V] rows of out_stride elements, or null
@@ -208,6 +221,9 @@ cudaError_t launch_gather_permute(const void* src, void* dst, int elem_bytes, si
 // aligned.  Same arithmetic as the prologue fused into the SIMT GEMV and the digit GEMV's prep.
 cudaError_t launch_prologue(int pro, const void* x, void* out, int dtype, const float* norm_w, float eps, size_t M,
                             size_t K, bool pdl, cudaStream_t stream);
+
+// The scratch of (current device, stream), grown to the sizes given; a status.
+int stream_scratch(size_t ws_floats, size_t counters, size_t act_bytes, int num_sms, cudaStream_t stream, TcScratch* out);
 
 // SM count and opt-in shared memory of the current device, as a status (B200Q8_ERR_UNSUPPORTED: not sm_100).
 int current_device(int* num_sms, size_t* max_smem);

@@ -2,6 +2,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <cstdlib>
 
 #include "b200q8.h"
 #include "kernels.h"
@@ -95,7 +96,18 @@ int linear_q4(const char* what, void* out, int out_dtype, const void* inp, int i
     a.group = group;
     a.in_dtype = in_dtype;
     a.out_dtype = out_dtype;
-    cudaError_t e = launch_q4_linear_generic(a, stream);
+    cudaError_t e;
+    static const int kGemmMin = getenv("Q4_GEMM") ? atoi(getenv("Q4_GEMM")) : 9;
+    if (M >= (size_t)kGemmMin && q4_gemm_tc_supports(a)) {
+        size_t ws = 0, counters = 0, act = 0;
+        q4_gemm_tc_scratch_need(a, sms, &ws, &counters, &act);
+        TcScratch scratch;
+        if ((st = stream_scratch(ws, counters, act, sms, stream, &scratch))) return st;
+        e = launch_q4_gemm_tc(a, sms, scratch, stream);
+        return e == cudaSuccess ? B200Q8_OK : cuda_fail(e, "q4_gemm launch");
+    }
+    e = launch_q4_stream(a, sms, smem, stream);
+    if (e == cudaErrorNotSupported) e = launch_q4_linear_generic(a, stream);
     return e == cudaSuccess ? B200Q8_OK : cuda_fail(e, "q4_linear launch");
 }
 

@@ -1,6 +1,8 @@
 // q4_gemv.cu -- 4-bit group-quantized weights times a few tokens.
 //
 // out[m, n] = sum_k x[m, k] * q[n, k] * s[n, k / group] (+ bias[n]) (+ res[m, n]), sums in fp32.
+#include <cooperative_groups.h>
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -10,6 +12,8 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "q4_common.cuh"
+#include "tc_utils.cuh"
+#include "tmap.cuh"
 
 namespace b200q8 {
 
@@ -75,7 +79,765 @@ cudaError_t launch_generic(const Q4Args& a, cudaStream_t stream)
     return e;
 }
 
+
+// ----------------------------------------------------------------------------------------------
+// Streaming kernel: K % 32 == 0, aligned pointers, up to 8 tokens.
+//
+// Exact integer products on the tensor cores.  A token's 128 consecutive elements ("chunk") become
+// integers X = rint(x * 2^(22 - e)), 2^e above the chunk's largest |x|, and X three signed bytes
+// X = 65536 X2 + 256 X1 + X0: three columns of the product.  The codes become bytes 16 q with three
+// integer operations per eight (one shift, two and-xor).  So mma.sync m16n8k32 (s8) sums 16 q * Xd
+// of a group exactly, and in fp32 every group's sum is multiplied by the group's scale and the
+// chunk's power of two and added to the row's.  What is rounded: an element to 2^-23 of its chunk's
+// largest (fp16 tokens are exact down to 2^-12 of it), and the fp32 sums, once a group.  A chunk that
+// holds an infinity or NaN is summed directly instead.  Chunks below 2^-100 count as below 2^-100.
+//
+// Why not fp16 operands: unpacking to fp16 takes 18 operations per 16 x 32 weights and two products,
+// to bytes 6 and one; on B200 (gate/up of a 7B model, 37888 x 3584, one token) the fp16 form of this
+// kernel ran at 17.9 us, bound by instruction issue.  Why not tcgen05: its operands would have to be
+// written back to shared or tensor memory as bytes, twice what was read; at 8 cycles a product, one
+// per three columns of 16 x 32 weights, mma.sync is within what HBM allows (about 44 cycles) to 13 tokens.
+//
+// Bound by HBM: half a byte a weight.
+//
+// Work: a tile is 16 rows; an item is a tile's next 256 or 512 of K.  `wk` warps share a tile (item ch
+// goes to warp ch mod wk) and add their sums through shared memory in warp order; a CTA of 8 or 16
+// warps has warps / wk such groups, each going through its own tiles.  Every warp has its own ring of
+// TMA copies ([16 rows x 128 bytes], 128-byte swizzle), running ahead across tile ends.  Tokens are put
+// into shared memory once per CTA.  Where a tile's K is split over a cluster's CTAs (few tiles, or
+// tokens too long for one CTA's shared memory), rank 0 adds the CTAs' sums from its shared memory in
+// rank order.  No workspace, no atomics: the result does not depend on timing.
+//
+// Which k a lane holds: within a group, lane t of a row's four takes group / 4 consecutive weights,
+// one shared load of 4, 8 or 16 bytes; a sum over k is in whatever order, as the tokens are laid
+// out to match.  Fragment row g is tile row rho(g), the bit reversal of g: with it the rows that one
+// phase of such a load touches differ in the swizzle's chunk, so there are no bank conflicts.
+//
+// A copy's wait is bounded: when it runs out the error word is set, the warp goes on without
+// waiting or copying (its outputs are invalid), and before it ends waits, bounded again, for the
+// copies it has in flight.
+constexpr int kMaxWarps = 16;
+constexpr int kBoxK = 256;  // K of one copied box: 128 bytes of each of 16 rows
+constexpr int kBoxBytes = 16 * 128;
+constexpr int kMaxStages = 4;
+constexpr int kMaxTokens = 8;
+constexpr uint64_t kWaitNs = 4000000000ull;  // far above any legitimate wait
+
+struct StreamParams {
+    Q4Args a;
+    int M;            // tokens of this launch
+    int wk, wk_log2;  // warps per tile
+    int stages;       // items in flight per warp
+    int nch;          // items per row
+    int per;          // items of one cluster rank
+    int tiles;
+};
+
+__device__ int g_q4_error;  // bit 0: a bounded wait ran out
+
+// Shared loads that the compiler may schedule: an address from `fence` keeps them behind a wait, and
+// `fence` on what was computed from them keeps them before the stage is given back.
+template <int W>
+__device__ __forceinline__ void lds(uint32_t a, uint32_t (&w)[W])
+{
+    static_assert(W == 1 || W == 2 || W == 4, "4, 8 or 16 bytes");
+    if constexpr (W == 1)
+        asm("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(a));
+    else if constexpr (W == 2)
+        asm("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
+    else
+        asm("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
+}
+__device__ __forceinline__ void fence(uint32_t& v) { asm volatile("" : "+r"(v)::"memory"); }
+__device__ __forceinline__ void fence(float& v) { asm volatile("" : "+f"(v)::"memory"); }
+
+// The eight codes of a word as bytes 16 q: elements 0, 2, 4, 6 and 1, 3, 5, 7.  (a & mask) ^ flip with the
+// flip turning q + 8 into the two's complement of q, in the upper half of each byte.
+__device__ __forceinline__ void unpack8(uint32_t w, uint32_t& even, uint32_t& odd)
+{
+    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(even) : "r"(w << 4), "r"(0xF0F0F0F0u), "r"(0x80808080u));
+    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(odd) : "r"(w), "r"(0xF0F0F0F0u), "r"(0x80808080u));
+}
+
+// d += A (16 x 32, s8, rows) * B (32 x 8, s8, columns); with kFirst d = `start` in every element + A * B
+template <bool kFirst>
+__device__ __forceinline__ void mma16832(int (&d)[4], int start, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1)
+{
+    if constexpr (kFirst)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(start));
+    else
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The sums start at the bit pattern of 1.5 * 2^23: read as a float they are that plus the sum, exact
+// while |sum| < 2^22 (a group's is at most 128 * 128 * 128 = 2^21).
+constexpr int kMagicBits = 0x4B400000;
+constexpr float kMagic = 12582912.0f;
+
+// Shared memory distance of two columns of `blocks` 32-blocks of bytes, two blocks to 64 bytes: an odd
+// number of those, so that neighbouring columns' loads fall into different banks.
+__host__ __device__ constexpr size_t column_stride(int blocks) { return (size_t)((blocks / 2) | 1) * 64; }
+
+// Columns of the product.  Up to two tokens: one 8-column tile, token m's byte d (X0, X1, X2) in column
+// 3 m + d.  Up to eight: three tiles, token m in column m of tile d.
+template <int NT>
+__device__ __forceinline__ int column_of(int m, int d, int M)  // where it is stored
+{
+    return NT == 1 ? 3 * m + d : d * M + m;
+}
+
+// Tokens into shared memory, `blocks` (a multiple of 8) 32-blocks from block0:
+//   xs      [column][pair of blocks][quarter t][2 blocks] of 8 bytes: the bytes that lane t multiplies
+//           with its word of a block, elements 0 2 4 6 1 3 5 7.  Within a group of W = group / 32 blocks, word
+//           w of lane t starts at element (t * W + w) * 8.  Zero behind K.
+//   weight  [chunk][8 NT]: what a column's integer counts, with the 1/16 of the codes' bytes
+//   direct  [token][chunk]: 1 if the chunk is summed directly; returns whether this thread saw any
+// Half a warp per chunk of 128 elements, eight elements a lane; a few chunks' loads at a time.  `then` is
+// called once the first loads are under way.
+template <int NT, class Then>
+__device__ __forceinline__ bool stage_tokens(unsigned char* xs, float* weight, unsigned char* direct,
+                                             const StreamParams& p, int W, int block0, int blocks, Then then)
+{
+    constexpr int U = 4;  // chunks whose loads are in flight
+    const int K = (int)p.a.K, chunks = blocks / 4;
+    const size_t cs = column_stride(blocks);
+    const int u = threadIdx.x & 15;  // word of the chunk
+    bool any = false;
+    const int total = chunks * p.M, half = threadIdx.x >> 4, halves = blockDim.x >> 4;
+    const bool f16 = p.a.in_dtype == kF16;
+    for (int i0 = half; i0 - half < total; i0 += U * halves) {  // whole warps: the shuffles below
+        uint4 raw[U][2];
+#pragma unroll
+        for (int q = 0; q < U; q++) {
+            const int i = i0 + q * halves, m = i / chunks, k = block0 * 32 + (i - m * chunks) * 128 + u * 8;
+            raw[q][0] = raw[q][1] = make_uint4(0, 0, 0, 0);
+            if (i < total && k < K) {
+                if (f16) {
+                    raw[q][0] = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.a.x) + (size_t)m * K + k);
+                } else {
+                    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(p.a.x) + (size_t)m * K + k);
+                    raw[q][0] = src[0];
+                    raw[q][1] = src[1];
+                }
+            }
+        }
+        if (i0 == half) then();
+#pragma unroll
+        for (int q = 0; q < U; q++) {
+            const int i = i0 + q * halves, m = i / chunks, c = i - m * chunks;
+            if (i - half >= total) break;  // uniform in the CTA
+            float v[8];
+            if (f16) {
+                const uint32_t h[4] = {raw[q][0].x, raw[q][0].y, raw[q][0].z, raw[q][0].w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+                    v[2 * j] = f.x, v[2 * j + 1] = f.y;
+                }
+            } else {
+                const uint4 lo = raw[q][0], hi = raw[q][1];
+                v[0] = __uint_as_float(lo.x), v[1] = __uint_as_float(lo.y), v[2] = __uint_as_float(lo.z);
+                v[3] = __uint_as_float(lo.w), v[4] = __uint_as_float(hi.x), v[5] = __uint_as_float(hi.y);
+                v[6] = __uint_as_float(hi.z), v[7] = __uint_as_float(hi.w);
+            }
+            uint32_t top = 0;  // largest |x| as bits: above every number for an infinity or NaN
+#pragma unroll
+            for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const bool bad = top >= 0x7F800000u;
+            const int e = max((int)(top >> 23) - 126, -100);  // |x| < 2^e
+            const float up = bad ? 0.0f : __uint_as_float((uint32_t)(22 - e + 127) << 23);
+            // X in the low bits of x * up + 1.5 * 2^23; with 128 added to each byte, the bytes are the signed
+            // digits with their top bit flipped.
+            uint32_t y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                y[j] = __float_as_uint(bad ? kMagic : fmaf(v[j], up, kMagic)) + (0x00808080u - (uint32_t)kMagicBits);
+            uint32_t d[3][2];  // digit, even / odd elements
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint32_t lo = __byte_perm(y[h], y[2 + h], 0x5140), hi = __byte_perm(y[4 + h], y[6 + h], 0x5140);
+                d[0][h] = __byte_perm(lo, hi, 0x5410) ^ 0x80808080u;
+                d[1][h] = __byte_perm(lo, hi, 0x7632) ^ 0x80808080u;
+                d[2][h] = __byte_perm(__byte_perm(y[h], y[2 + h], 0x0062), __byte_perm(y[4 + h], y[6 + h], 0x0062), 0x5410) ^ 0x80808080u;
+            }
+            const int o = u & (4 * W - 1), b = c * 4 + u / (4 * W) * W + (o & (W - 1)), t = o / W;
+            unsigned char* dst = xs + (b >> 1) * 64 + t * 16 + (b & 1) * 8;
+            if (i < total) {
+#pragma unroll
+                for (int n = 0; n < 3; n++)
+                    *reinterpret_cast<uint2*>(dst + column_of<NT>(m, n, p.M) * cs) = make_uint2(d[n][0], d[n][1]);
+                if (u < 3)
+                    weight[c * 8 * NT + (NT == 1 ? 3 * m + u : 8 * u + m)] =
+                        __uint_as_float((uint32_t)(e - 22 - 4 + 8 * u + 127) << 23);
+                if (u == 3) direct[m * chunks + c] = bad;
+                any |= bad;
+            }
+        }
+    }
+    return any;
+}
+
+// A warp adds to sums[r], r < 16, token m's products with rows tile * 16 + r over 128-chunk c, as the formula
+// reads: what infinities and NaN need.
+__device__ __noinline__ void direct_chunk(const Q4Args& a, float* sums, int tile, int m, int c)
+{
+    const int lane = threadIdx.x & 31;
+    const size_t K = a.K, ng = (K + a.group - 1) / a.group;
+    for (int r = 0; r < 16; r++) {
+        const size_t n = (size_t)tile * 16 + r;
+        if (n >= a.N) break;
+        float v = 0.0f;
+        for (int j = lane; j < 64; j += 32) {
+            const size_t k = (size_t)c * 128 + 2 * j;
+            if (k >= K) break;
+            const float s = bf16_bits_to_f32(a.scales[n * ng + k / a.group]);
+            const int code = a.q4[(n * K + k) / 2];
+            const size_t i = (size_t)m * K + k;
+            const float x0 = a.in_dtype == kF16 ? __half2float(static_cast<const __half*>(a.x)[i])
+                                                : static_cast<const float*>(a.x)[i];
+            const float x1 = a.in_dtype == kF16 ? __half2float(static_cast<const __half*>(a.x)[i + 1])
+                                                : static_cast<const float*>(a.x)[i + 1];
+            v = fmaf((float)((code & 15) - 8) * s, x0, v);
+            v = fmaf((float)((code >> 4) - 8) * s, x1, v);
+        }
+        v = warp_sum(v);
+        if (lane == 0) sums[r] += v;
+    }
+    __syncwarp();
+}
+
+template <int NT, int IB>
+struct StreamCfg {
+    static constexpr int kItemBytes = IB * kBoxBytes;
+    static constexpr int kChunks = IB * kBoxK / 128;  // 128-chunks of an item
+    static constexpr int kCols = 8 * NT;              // columns kept in `weight`
+    static constexpr int kSums = NT == 1 ? 2 * 16 : 8 * 16;  // a tile's outputs: [token][row]
+    static size_t smem(int warps, int stages, int M, int per, int cluster)
+    {
+        const int chunks = per * kChunks;
+        return 1024 + (size_t)warps * stages * kItemBytes + warps * kMaxStages * 8 + 3 * M * column_stride(chunks * 4) +
+               (size_t)chunks * kCols * 4 + (size_t)2 * warps * kSums * 4 +
+               (cluster > 1 ? (size_t)2 * cluster * kSums * 4 : 0) + (size_t)M * chunks;
+    }
+};
+
+template <int NT, int G, int IB>
+__global__ void __launch_bounds__(kMaxWarps * 32, 1)
+    q4_stream_kernel(const __grid_constant__ CUtensorMap tmW, const StreamParams p)
+{
+    using C = StreamCfg<NT, IB>;
+    constexpr int kItemBytes = C::kItemBytes;
+    constexpr int W = G / 32;   // words a lane holds of a group; 32-blocks of a group
+    constexpr int GC = 128 / G;  // groups of a chunk
+    namespace cg = cooperative_groups;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int csize = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int warps = blockDim.x >> 5;
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) &
+                                                           ~static_cast<uintptr_t>(1023));
+    const int ch0 = rank * p.per, ch1 = min(p.nch, ch0 + p.per);  // items of a row that this CTA takes
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (size_t)warps * p.stages * kItemBytes);
+    unsigned char* xs = reinterpret_cast<unsigned char*>(bars + warps * kMaxStages);
+    const int xchunks = p.per * C::kChunks;
+    const size_t cs = column_stride(xchunks * 4);
+    float* weight = reinterpret_cast<float*>(xs + 3 * p.M * cs);
+    float* red = weight + xchunks * C::kCols;         // [2][warp][tile's outputs]
+    float* cbuf = red + 2 * warps * C::kSums;         // [2][rank][tile's outputs] of a cluster's CTAs (in rank 0)
+    unsigned char* direct = reinterpret_cast<unsigned char*>(cbuf + (csize > 1 ? 2 * csize * C::kSums : 0));
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+    const int row = ((g & 1) << 2) | (g & 2) | (g >> 2);  // rho(g); the fragment's other row is row + 8
+    const int wk = p.wk, kw = warp & (wk - 1);
+    const int group = warp >> p.wk_log2, groups = warps >> p.wk_log2;
+    const int tbase = ((int)blockIdx.x / csize) * groups, tile0 = tbase + group;
+    const int tstep = ((int)gridDim.x / csize) * groups;
+    const int N = (int)p.a.N, K = (int)p.a.K;
+    const int ng = (K + G - 1) / G;
+
+    // ---- copies: the warp's items in order, (tile, ch) with ch = ch0 + kw, + wk, ...
+    const uint32_t ring = tc::smem_u32(smem) + warp * p.stages * kItemBytes;
+    const uint32_t bar0 = tc::smem_u32(bars + warp * kMaxStages);
+    const bool busy = ch0 + kw < ch1;  // there are items for this warp
+    int itile = busy ? tile0 : p.tiles, ich = ch0 + kw, inflight = 0;
+    auto advance = [&]() {
+        ich += wk;
+        if (ich >= ch1) {
+            ich = ch0 + kw;
+            itile += tstep;
+        }
+    };
+    // A tile's scales, 16 rows' worth and contiguous, into L2 ahead of their loads.
+    auto prefetch_scales = [&](int tile) {
+        const size_t off = (size_t)tile * 16 * ng;
+        const uint32_t bytes = (uint32_t)(min(16, N - tile * 16) * ng * 2) & ~15u;
+        if (bytes && ((uintptr_t)p.a.scales & 15) == 0)
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.a.scales + off), "r"(bytes) : "memory");
+    };
+    if (lane == 0) {
+        for (int i = 0; i < p.stages; i++) tc::mbar_init(bar0 + 8 * i, 1);
+        tc::fence_mbar_init();
+        tc::prefetch_tensormap(&tmW);
+        // While the kernel before ends: this warp's first item into L2.  (Into L2 only, where it stays
+        // coherent: the kernel before may have written the weights themselves.)
+        if (kw == 0 && tile0 < p.tiles) prefetch_scales(tile0);
+        if (itile < p.tiles)
+            for (int b = 0; b < IB; b++) tc::tma_prefetch_l2_2d(&tmW, (ich * IB + b) * 128, itile * 16);
+    }
+    pdl_wait();
+    pdl_launch_dependents();
+    const uint64_t policy = tc::l2_policy_evict_first();
+    auto load_item = [&](int stage) {
+        tc::mbar_arrive_expect_tx(bar0 + 8 * stage, kItemBytes);
+#pragma unroll
+        for (int b = 0; b < IB; b++)  // behind a row's end or the last row: zeros
+            tc::tma_load_2d_hint(ring + stage * kItemBytes + b * kBoxBytes, &tmW, (ich * IB + b) * 128, itile * 16,
+                                 bar0 + 8 * stage, policy);
+    };
+    // Scales of the chunk about to be multiplied, loaded while the one before is.
+    uint32_t sc0[GC], sc1[GC];
+    const uint16_t *sp0 = nullptr, *sp1 = nullptr;
+    int sg = 0;  // group index that sp0, sp1 point at
+    auto load_scales = [&]() {
+        if (sg + GC <= ng) {
+#pragma unroll
+            for (int i = 0; i < GC; i++) sc0[i] = __ldg(sp0 + i), sc1[i] = __ldg(sp1 + i);
+        } else {  // a row's last item may be short
+#pragma unroll
+            for (int i = 0; i < GC; i++) {
+                const bool in = sg + i < ng;
+                sc0[i] = in ? (uint32_t)__ldg(sp0 + i) : 0u;
+                sc1[i] = in ? (uint32_t)__ldg(sp1 + i) : 0u;
+            }
+        }
+    };
+    auto first_scales = [&](int tile) {
+        sg = (ch0 + kw) * C::kChunks * GC;
+        sp0 = p.a.scales + (size_t)min(tile * 16 + row, N - 1) * ng + sg;
+        sp1 = p.a.scales + (size_t)min(tile * 16 + row + 8, N - 1) * ng + sg;
+        load_scales();
+    };
+    // The tokens' loads go first and one item a warp behind them, the others once the tokens are done: behind
+    // more the loads would wait for megabytes to pass (37888 x 3584, one token: 14.9 us; all items first 16.5).
+    const bool some = stage_tokens<NT>(xs, weight, direct, p, W, ch0 * C::kChunks * 4, xchunks * 4, [&]() {
+        if (lane == 0 && itile < p.tiles) {
+            load_item(inflight++);
+            advance();
+        }
+        if (busy && tile0 < p.tiles) first_scales(tile0);
+    });
+    if (lane == 0)
+        for (; inflight < p.stages && itile < p.tiles; inflight++, advance()) load_item(inflight);
+    const bool any_direct = __syncthreads_or(some);
+    if (csize > 1) cluster.sync();  // every rank runs before rank 0's memory is stored to
+
+    uint32_t xoff[NT];  // this lane's column of each 8-column tile (lanes behind the last column repeat it)
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+        xoff[nt] = tc::smem_u32(xs) + t * 16 +
+                   (uint32_t)((NT == 1 ? min(g, 3 * p.M - 1) : nt * p.M + min(g, p.M - 1)) * cs);
+    // The lane's words of group 0 of a box: 16-byte piece ((t * W) / 4) ^ row of its row; another group is an
+    // XOR away.
+    const uint32_t wlane = row * 128 + ((((t * W) >> 2) ^ row) << 4) + ((t * W) & 3) * 4;
+
+    const int zero = 0;
+    bool ok = true;
+    int stage = 0, parity = 0;
+    uint32_t phase = 0;
+    const int rounds = (p.tiles - tbase + tstep - 1) / tstep;  // uniform in a cluster
+    for (int it = 0; it < rounds; it++) {
+        const int tile = tile0 + it * tstep;
+        if (tile >= p.tiles) break;  // groups end on their own; with a cluster there is one group
+        if (lane == 0 && kw == 0 && tile + tstep < p.tiles) prefetch_scales(tile + tstep);
+        float acc[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[nt][i] = 0.0f;
+        for (int ch = ch0 + kw; ch < ch1; ch += wk) {
+            if (ok) {
+                ok = __all_sync(0xffffffffu, tc::mbar_wait(bar0 + 8 * stage, phase, &zero, kWaitNs));
+                if (!ok && lane == 0) atomicOr(&g_q4_error, 1);
+            }
+            uint32_t wrow = ring + stage * kItemBytes + wlane;
+            fence(wrow);
+            uint32_t xitem = (uint32_t)(ch - ch0) * (C::kChunks * 128);
+            const float* wchunk = weight + (ch - ch0) * C::kChunks * C::kCols + 2 * t;
+            // Chunks behind K need no care: their codes and tokens are zeros, and so are their scales.
+#pragma unroll 1
+            for (int c = 0; c < C::kChunks; c++) {
+                float s0[GC], s1[GC];
+#pragma unroll
+                for (int i = 0; i < GC; i++) s0[i] = bf16_bits_to_f32(sc0[i]), s1[i] = bf16_bits_to_f32(sc1[i]);
+                if (c + 1 < C::kChunks) {
+                    sp0 += GC, sp1 += GC, sg += GC;
+                    load_scales();
+                } else if (ch + wk < ch1) {
+                    const int step = ((wk - 1) * C::kChunks + 1) * GC;
+                    sp0 += step, sp1 += step, sg += step;
+                    load_scales();
+                } else if (tile + tstep < p.tiles) {
+                    first_scales(tile + tstep);
+                }
+                uint32_t x[NT][2][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    lds<4>(xoff[nt] + xitem, x[nt][0]);
+                    lds<4>(xoff[nt] + xitem + 64, x[nt][1]);
+                }
+                float sum[NT][4];
+#pragma unroll
+                for (int gi = 0; gi < GC; gi++) {
+                    uint32_t w0[W], w1[W];
+                    lds<W>(wrow ^ (gi * W * 16), w0);
+                    lds<W>((wrow ^ (gi * W * 16)) + 1024, w1);
+                    int d[NT][4];
+#pragma unroll
+                    for (int b = 0; b < W; b++) {
+                        const int blk = gi * W + b;
+                        uint32_t a0, a1, a2, a3;
+                        unpack8(w0[b], a0, a2);
+                        unpack8(w1[b], a1, a3);
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            const uint32_t b0 = x[nt][blk >> 1][2 * (blk & 1)], b1 = x[nt][blk >> 1][2 * (blk & 1) + 1];
+                            if (b == 0)
+                                mma16832<true>(d[nt], kMagicBits, a0, a1, a2, a3, b0, b1);
+                            else
+                                mma16832<false>(d[nt], 0, a0, a1, a2, a3, b0, b1);
+                        }
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float f = __int_as_float(d[nt][i]) - kMagic, r = i < 2 ? s0[gi] : s1[gi];
+                            sum[nt][i] = gi == 0 ? f * r : fmaf(f, r, sum[nt][i]);
+                        }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    const float2 wt = *reinterpret_cast<const float2*>(wchunk + nt * 8);
+                    acc[nt][0] = fmaf(sum[nt][0], wt.x, acc[nt][0]);
+                    acc[nt][1] = fmaf(sum[nt][1], wt.y, acc[nt][1]);
+                    acc[nt][2] = fmaf(sum[nt][2], wt.x, acc[nt][2]);
+                    acc[nt][3] = fmaf(sum[nt][3], wt.y, acc[nt][3]);
+                }
+                wrow ^= 64;  // a box's other chunk
+                if (c & 1) wrow += kBoxBytes;
+                xitem += 128;
+                wchunk += C::kCols;
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) fence(acc[nt][i]);
+            __syncwarp();  // the stage is read
+            if (ok) {  // else the ring stays as it is, for the end
+                if (lane == 0) {
+                    inflight--;
+                    if (itile < p.tiles) {
+                        load_item(stage);
+                        inflight++;
+                        advance();
+                    }
+                }
+                if (++stage == p.stages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+        // ---- a token's three columns: v[i] of rows row (i < 2) and row + 8, tokens mt and mt + 1 (NT == 1: mt only)
+        float v[4];
+        int mt;
+        if constexpr (NT == 1) {  // columns 0 1 | 2, 3 | 4 5 of lanes t = 0, 1, 2
+            const float a = __shfl_down_sync(0xffffffffu, acc[0][0], 1), b = __shfl_down_sync(0xffffffffu, acc[0][2], 1);
+            const float c = __shfl_up_sync(0xffffffffu, acc[0][1], 1), d = __shfl_up_sync(0xffffffffu, acc[0][3], 1);
+            mt = t >> 1;
+            v[0] = t == 0 ? acc[0][0] + acc[0][1] + a : c + acc[0][0] + acc[0][1];
+            v[2] = t == 0 ? acc[0][2] + acc[0][3] + b : d + acc[0][2] + acc[0][3];
+            v[1] = v[3] = 0.0f;
+        } else {
+            mt = 2 * t;
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = acc[0][i] + acc[1][i] + acc[2][i];
+        }
+        auto mine = [&](int i) {  // whether v[i] is an output's sum
+            return NT == 1 ? (t & 1) == 0 && (i & 1) == 0 && mt < p.M : mt + (i & 1) < p.M;
+        };
+        auto put = [&](int m, int r, float y) {
+            const long long n = (long long)tile * 16 + r;
+            if (n >= N) return;
+            const long long o = (long long)m * N + n;
+            if (p.a.out_dtype == kF16)
+                q4_store<__half>(static_cast<__half*>(p.a.out) + o,
+                                 p.a.res ? static_cast<const __half*>(p.a.res) + o : nullptr, y, p.a.bias, n);
+            else
+                q4_store<float>(static_cast<float*>(p.a.out) + o, p.a.res ? static_cast<const float*>(p.a.res) + o : nullptr,
+                                y, p.a.bias, n);
+        };
+        if (wk == 1 && !any_direct) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (mine(i)) put(mt + (i & 1), row + 8 * (i >> 1), v[i]);
+            continue;
+        }
+        // ---- the tile's sums: warps in order, then cluster ranks in order
+        float* rbuf = red + parity * warps * C::kSums;
+        float* wsum = rbuf + warp * C::kSums;  // [token][row]
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (mine(i)) wsum[(mt + (i & 1)) * 16 + row + 8 * (i >> 1)] = v[i];
+        if (any_direct) {  // rare: infinities or NaN among this CTA's elements
+            __syncwarp();
+            for (int m = 0; m < p.M; m++)
+                for (int c = kw; c < xchunks; c += wk)
+                    if (direct[m * xchunks + c]) direct_chunk(p.a, wsum + m * 16, tile, m, ch0 * C::kChunks + c);
+        }
+        if (wk == 1)
+            __syncwarp();
+        else
+            asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(wk * 32) : "memory");
+        const int gt = kw * 32 + lane, outs = p.M * 16;
+        const float* gsum = rbuf + group * wk * C::kSums;
+        auto warp_sums = [&](int e) {
+            float y = gsum[e];
+#pragma unroll 4
+            for (int w = 1; w < wk; w++) y += gsum[w * C::kSums + e];
+            return y;
+        };
+        if (csize == 1) {
+            for (int e = gt; e < outs; e += wk * 32) put(e >> 4, e & 15, warp_sums(e));
+        } else {
+            // Rank 0 collects.  The others go on and wait for this tile's barrier before they store for the
+            // next: by then rank 0 has read what their buffer held two tiles ago.
+            if (it > 0 && rank != 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+            float* to = cluster.map_shared_rank(cbuf, 0) + (parity * csize + rank) * C::kSums;
+            for (int e = gt; e < outs; e += wk * 32) to[e] = warp_sums(e);
+            __syncwarp();
+            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+            if (rank == 0) {
+                asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+                const float* from = cbuf + parity * csize * C::kSums;
+                for (int e = gt; e < outs; e += wk * 32) {
+                    float y = from[e];
+                    for (int c = 1; c < csize; c++) y += from[c * C::kSums + e];
+                    put(e >> 4, e & 15, y);
+                }
+                __syncwarp();
+            }
+        }
+        parity ^= 1;  // one buffer is read while the next tile's sums go to the other
+    }
+    if (!ok && lane == 0)  // copies still in flight land before the CTA ends
+        for (int i = 0; i < inflight; i++) {
+            tc::mbar_wait(bar0 + 8 * stage, phase, &zero, kWaitNs);
+            if (++stage == p.stages) stage = 0, phase ^= 1;
+        }
+    if (csize > 1) {
+        if (rounds > 0 && rank != 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster.sync();  // rank 0's memory outlives the stores into it
+    }
+}
+
+constexpr size_t kSmemPerSM = 228 * 1024;
+
+struct StreamPlan {
+    int tokens = 0;  // of one launch; 0: the kernel cannot take the shape
+    int nt = 0, ib = 1, cluster = 1, nch = 0, per = 0, warps = 8, wk = 8, stages = 0;
+};
+
+template <int NT, int G, int IB>
+cudaError_t launch_stream(const StreamParams& p, const StreamPlan& s, int num_sms, size_t max_smem, cudaStream_t stream)
+{
+    using C = StreamCfg<NT, IB>;
+    CUtensorMap mw;
+    TmapDesc w{};
+    w.base = p.a.q4;
+    w.inner = p.a.K / 2;
+    w.outer = p.a.N;
+    w.row_bytes = p.a.K / 2;
+    w.box_inner = 128;
+    w.box_outer = 16;
+    w.dtype = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    w.swizzle = CU_TENSOR_MAP_SWIZZLE_128B;
+    if (!tmap_2d(&mw, w)) return cudaErrorInvalidValue;
+    auto kern = q4_stream_kernel<NT, G, IB>;
+    static thread_local bool configured[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!configured[dev]) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)max_smem);
+        if (e != cudaSuccess) return e;
+        configured[dev] = true;
+    }
+    const int groups = s.warps / p.wk;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3((unsigned)s.warps * 32);
+    cfg.dynamicSmemBytes = C::smem(s.warps, p.stages, p.M, p.per, s.cluster);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)s.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = s.cluster > 1 ? 2 : 1;
+    // As many CTAs (clusters) as the device holds at a time.  The hardware's own count: a cluster stays
+    // within a GPC, so fewer fit than the SMs would hold.
+    int resident = (s.warps == 8 && 2 * cfg.dynamicSmemBytes + 2048 <= kSmemPerSM ? 2 : 1) * num_sms;
+    if (s.cluster > 1) {
+        struct Known {
+            int dev, cluster, warps, n;
+            size_t smem;
+        };
+        static thread_local Known known[16];
+        static thread_local int used = 0, next = 0;
+        int i = 0;
+        while (i < used && !(known[i].dev == dev && known[i].cluster == s.cluster && known[i].warps == s.warps &&
+                             known[i].smem == cfg.dynamicSmemBytes))
+            i++;
+        if (i == used) {
+            Known k{dev, s.cluster, s.warps, 0, cfg.dynamicSmemBytes};
+            cfg.gridDim = dim3((unsigned)s.cluster);
+            cfg.attrs = attr + 1;
+            cfg.numAttrs = 1;
+            if ((e = cudaOccupancyMaxActiveClusters(&k.n, kern, &cfg)) != cudaSuccess) return e;
+            cfg.attrs = attr;
+            cfg.numAttrs = 2;
+            i = used < 16 ? used++ : next++ % 16;
+            known[i] = k;
+        }
+        resident = std::max(1, known[i].n);
+    }
+    cfg.gridDim = dim3((unsigned)(std::min((p.tiles + groups - 1) / groups, resident) * s.cluster));
+    e = cudaLaunchKernelEx(&cfg, kern, mw, p);
+    if (e == cudaSuccess) note_launch();
+    return e;
+}
+
+template <int G>
+cudaError_t launch_stream_nt(const StreamParams& p, const StreamPlan& s, int num_sms, size_t max_smem, cudaStream_t stream)
+{
+    if (s.nt == 1)
+        return s.ib == 1 ? launch_stream<1, G, 1>(p, s, num_sms, max_smem, stream)
+                         : launch_stream<1, G, 2>(p, s, num_sms, max_smem, stream);
+    return launch_stream<3, G, 1>(p, s, num_sms, max_smem, stream);
+}
+
+size_t stream_smem(int nt, int ib, int warps, int stages, int M, int per, int cluster)
+{
+    if (nt == 1)
+        return ib == 1 ? StreamCfg<1, 1>::smem(warps, stages, M, per, cluster) : StreamCfg<1, 2>::smem(warps, stages, M, per, cluster);
+    return StreamCfg<3, 1>::smem(warps, stages, M, per, cluster);
+}
+
+constexpr int kMaxCluster = 8;
+
+StreamPlan plan_stream(const Q4Args& a, size_t M, int num_sms, size_t max_smem)
+{
+    StreamPlan s;
+    const int tiles = (int)((a.N + 15) / 16);
+    for (int m = (int)std::min<size_t>(M, kMaxTokens); m >= 1 && !s.tokens; m--) {
+        const int nt = m <= 2 ? 1 : 3;
+        const int ib = a.K >= 2048 && nt == 1 ? 2 : 1;
+        const int nch = (int)((a.K + ib * kBoxK - 1) / (ib * kBoxK));
+        for (int c = 1; c <= kMaxCluster && !s.tokens; c *= 2) {
+            const int per = (nch + c - 1) / c;
+            if ((nch + per - 1) / per != c) continue;  // a rank would have nothing
+            auto fit = [&](int warps, size_t budget) {
+                int st = ib == 2 ? 2 : 3;
+                while (st >= 2 && stream_smem(nt, ib, warps, st, m, per, c) > budget) st--;
+                return st;
+            };
+            int warps = 8, stages = fit(8, kSmemPerSM / 2 - 1024);  // two CTAs of 8 warps an SM
+            if (stages < 2) stages = fit(warps = 16, max_smem);      // one of 16
+            if (stages < 2) stages = fit(warps = 8, max_smem);       // or of 8
+            if (stages < 2) continue;
+            s.tokens = m;
+            s.nt = nt;
+            s.ib = ib;
+            s.nch = nch;
+            s.cluster = c;
+            s.per = per;
+            s.warps = warps;
+            s.stages = stages;
+        }
+    }
+    if (!s.tokens) return s;
+    s.wk = s.warps;
+    if (s.cluster == 1) {
+        const int slots = num_sms * 16;
+        double best = 1e30;
+        for (int wk = 1; wk <= s.warps; wk *= 2) {
+            const double cost = (double)(((long long)tiles * wk + slots - 1) / slots) * ((s.nch + wk - 1) / wk + (wk == 1 ? 0.5 : 1.0));
+            if (cost < best) best = cost, s.wk = wk;
+        }
+    }
+    return s;
+}
+
 }  // namespace
+
+bool q4_stream_supports(const Q4Args& a)
+{
+    return a.K % 32 == 0 && (uintptr_t)a.q4 % 16 == 0 && (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.scales % 4 == 0 &&
+           a.N <= (size_t)INT32_MAX - 4096 && encode_fn() != nullptr;
+}
+
+cudaError_t launch_q4_stream(const Q4Args& a, int num_sms, size_t max_smem, cudaStream_t stream)
+{
+    if (!q4_stream_supports(a)) return cudaErrorNotSupported;
+    const size_t ib = a.in_dtype == kF16 ? 2 : 4, ob = a.out_dtype == kF16 ? 2 : 4;
+    const StreamPlan first = plan_stream(a, a.M, num_sms, max_smem);
+    if (!first.tokens) return cudaErrorNotSupported;  // one token's slice exceeds the shared memory
+    for (size_t m0 = 0; m0 < a.M;) {
+        const StreamPlan s = plan_stream(a, std::min<size_t>(a.M - m0, (size_t)first.tokens), num_sms, max_smem);
+        StreamParams p;
+        p.a = a;
+        p.a.x = static_cast<const char*>(a.x) + m0 * a.K * ib;
+        p.a.out = static_cast<char*>(a.out) + m0 * a.N * ob;
+        p.a.res = a.res ? static_cast<const char*>(a.res) + m0 * a.N * ob : nullptr;
+        p.M = s.tokens;
+        p.wk = s.wk;
+        p.wk_log2 = s.wk == 16 ? 4 : s.wk == 8 ? 3 : s.wk == 4 ? 2 : s.wk == 2 ? 1 : 0;
+        p.stages = s.stages;
+        p.nch = s.nch;
+        p.per = s.per;
+        p.tiles = (int)((a.N + 15) / 16);
+        cudaError_t e = a.group == 32   ? launch_stream_nt<32>(p, s, num_sms, max_smem, stream)
+                        : a.group == 64 ? launch_stream_nt<64>(p, s, num_sms, max_smem, stream)
+                                        : launch_stream_nt<128>(p, s, num_sms, max_smem, stream);
+        if (e != cudaSuccess) return e;
+        m0 += (size_t)s.tokens;
+    }
+    return cudaSuccess;
+}
+
+cudaError_t read_kernel_error_q4(int* code, bool clear)
+{
+    int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, g_q4_error, sizeof(int));
+    if (e != cudaSuccess) return e;
+    *code = v;
+    if (clear && v) {
+        const int z = 0;
+        e = cudaMemcpyToSymbol(g_q4_error, &z, sizeof(int));
+    }
+    return e;
+}
 
 cudaError_t launch_q4_linear_generic(const Q4Args& a, cudaStream_t stream)
 {

@@ -45,6 +45,12 @@
 //          or the stream-K partial/fixup path;
 //   14     (two-issuer layouts) a second thread issuing the MMAs of every other
 //          stage into its own accumulator; the epilogue adds the two.
+// The same kernel takes 4-bit weights with a scale per group (q4_common.cuh): the tile's rows are half
+// as many bytes, and the dequantizers write q * s, exact in fp16 once a row's scales are divided by a
+// power of two of their own (q4_scale_prep_kernel below, whose power of two becomes the row's scale in
+// the epilogue): q * s has 3 + 8 significant bits, and groups down to 2^-29 of their row's largest scale
+// keep all of them.
+//
 // Every mbarrier wait is bounded (wall clock); a timeout sets a device error
 // word, drains in-flight copies and MMAs, frees TMEM and returns.  No TMA
 // multicast and no thread-block clusters are used.
@@ -94,6 +100,12 @@ __device__ unsigned long long g_gemm_role[1024][16];
 namespace {
 
 constexpr int kTileRows = 128;  // weight rows per tile (UMMA M)
+
+// 4-bit weights: what q4_scale_prep_kernel made of their scales.
+struct Q4Scales {
+    const __half* gs = nullptr;  // [groups][ld]
+    int ld = 0, group_log2 = 0, groups = 0;
+};
 constexpr int kFirstConv = 2, kFirstEpi = 10;
 constexpr int kSecondIssuer = 14;  // warp of the second MMA-issuing thread (two-issuer layouts)
 constexpr uint64_t kWaitTimeoutNs = 4000000000ull;  // 4 s: far above any legitimate wait
@@ -125,14 +137,18 @@ struct SkParams {
     long long units;    // tiles * kbpt
     int tma_out;        // outputs leave by TMA store (16-byte aligned rows), else direct stores
     int w_evict_first;  // weight tiles are read by one token tile only: L2 evict-first
+    const __half* gs;   // 4-bit weights: [groups][gs_ld] normalized group scales
+    int gs_ld, group_log2, groups;
 };
 
-template <int BN, int BK, int S, int SA, int NI>
+// WB: bits of a weight, 8 or 4.
+template <int BN, int BK, int S, int SA, int NI, int WB = 8>
 struct SkCfg {
-    static constexpr int kWBoxW = BK < 128 ? BK : 128;  // bytes per weight-box row
-    static constexpr int kWBoxes = BK / kWBoxW;
+    static constexpr int kRowBytes = BK * WB / 8;       // bytes of a weight row in one stage
+    static constexpr int kWBoxW = kRowBytes < 128 ? kRowBytes : 128;  // bytes per weight-box row
+    static constexpr int kWBoxes = kRowBytes / kWBoxW;
     static constexpr int kWBoxBytes = kTileRows * kWBoxW;
-    static constexpr int kW8Bytes = kTileRows * BK;
+    static constexpr int kW8Bytes = kTileRows * kRowBytes;
     static constexpr int kXBoxes = BK / 64;             // [BN rows x 64 fp16] boxes per stage
     static constexpr int kXBoxBytes = BN * 128;
     static constexpr int kXBytes = kXBoxes * kXBoxBytes;
@@ -165,14 +181,30 @@ struct SkCfg {
 };
 
 // Byte offset of 16-byte chunk c of row r inside a weight box, under the box's
-// TMA swizzle (128-byte rows: chunk ^= r & 7; 64-byte rows: chunk ^= (r >> 1) & 3).
+// TMA swizzle (128-byte rows: chunk ^= r & 7; 64-byte rows: chunk ^= (r >> 1) & 3; 32-byte rows:
+// chunk ^= (r >> 2) & 1).
 template <int kBoxW>
 __device__ __forceinline__ int wchunk(int r, int c)
 {
     if constexpr (kBoxW == 128)
         return r * 128 + ((c ^ (r & 7)) << 4);
-    else
+    else if constexpr (kBoxW == 64)
         return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+    else
+        return r * 32 + ((c ^ ((r >> 2) & 1)) << 4);
+}
+
+// The eight 4-bit codes of a word times `s` as four packed pairs, elements (0,1), (2,3), (4,5), (6,7).  A byte
+// goes into both halves of a pair above 2^10, of which one keeps the low and the other the high
+// (16 times) nibble; one packed fma leaves the integers q, one multiplication q * s.
+__device__ __forceinline__ void q4x8_to_h2x4(uint32_t w, uint32_t s, uint32_t* h)
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        h[i] = __byte_perm(w, 0x64646464u, 0x4040 + 0x0101 * i) & 0x64F0640Fu;  // 1024 + n0, 1024 + 16 n1
+        asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(h[i]) : "r"(0x2C003C00u), "r"(0xD480E408u));  // - 1032; / 16 - 72
+        asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[i]) : "r"(s));
+    }
 }
 
 __device__ __forceinline__ void raise_error(volatile int* abort)
@@ -259,12 +291,12 @@ __device__ __forceinline__ void tmem_ld_chunk(uint32_t col, float (&v)[CH])
     }
 }
 
-template <int BN, int BK, int S, int SA, int NI, typename OT>
-__global__ void __launch_bounds__(SkCfg<BN, BK, S, SA, NI>::kThreads, 1)
+template <int BN, int BK, int S, int SA, int NI, int WB, typename OT>
+__global__ void __launch_bounds__(SkCfg<BN, BK, S, SA, NI, WB>::kThreads, 1)
     q8_gemm_sk_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                       const __grid_constant__ CUtensorMap tmO, const SkParams p)
 {
-    using C = SkCfg<BN, BK, S, SA, NI>;
+    using C = SkCfg<BN, BK, S, SA, NI, WB>;
     constexpr int CH = C::kChunk;
     constexpr int kRedSlotBytes = kTileRows * CH * 4;  // one piece's CH-column chunk
     constexpr int kRedSlots = S * (C::kW8Bytes + C::kXBytes) / kRedSlotBytes;
@@ -327,8 +359,8 @@ __global__ void __launch_bounds__(SkCfg<BN, BK, S, SA, NI>::kThreads, 1)
                 tc::mbar_arrive_expect_tx(fb, C::kW8Bytes + C::kXBytes);
 #pragma unroll
                 for (int h = 0; h < C::kWBoxes; h++)
-                    tc::tma_load_2d(sw_base + pre * C::kW8Bytes + h * C::kWBoxBytes, &tmW, kb * BK + h * C::kWBoxW,
-                                    row0, fb);
+                    tc::tma_load_2d(sw_base + pre * C::kW8Bytes + h * C::kWBoxBytes, &tmW,
+                                    kb * C::kRowBytes + h * C::kWBoxW, row0, fb);
             }
         }
     }
@@ -376,7 +408,7 @@ __global__ void __launch_bounds__(SkCfg<BN, BK, S, SA, NI>::kThreads, 1)
 #pragma unroll
                         for (int h = 0; h < C::kWBoxes; h++)
                             tc::tma_load_2d_hint(sw_base + st.idx * C::kW8Bytes + h * C::kWBoxBytes, &tmW,
-                                                 kb * BK + h * C::kWBoxW, row0, fb, wpol);
+                                                 kb * C::kRowBytes + h * C::kWBoxW, row0, fb, wpol);
                     }
                     const uint32_t xdst = sx_base + st.idx * C::kXBytes;
 #pragma unroll
@@ -478,6 +510,17 @@ __global__ void __launch_bounds__(SkCfg<BN, BK, S, SA, NI>::kThreads, 1)
         while (ok && it.next(t, k0, k1)) {
             for (int kb = k0; kb < k1; kb++, g++, st.next(S), sa.next(SA)) {
                 if ((g & 1) != group) continue;
+                // 4-bit weights: this row's scale of every 32 weights of the stage (a group is one, two or four
+                // times 32; behind K the weights meet zero activations)
+                uint32_t gsv[WB == 4 ? BK / 32 : 1];
+                if constexpr (WB == 4) {
+                    const __half* gp = p.gs + (t % p.tiles_n) * kTileRows + r;
+#pragma unroll
+                    for (int c = 0; c < BK / 32; c++) {
+                        const int gi = min((kb * BK + c * 32) >> p.group_log2, p.groups - 1);
+                        gsv[c] = __half_as_ushort(__ldg(gp + (size_t)gi * p.gs_ld));
+                    }
+                }
                 ok = __all_sync(0xffffffffu, timed_wait(full0 + 8u * st.idx, st.phase, abort, w_full));
                 if (!ok) break;
                 if (g >= SA) {  // the MMAs that read this A stage last are done
@@ -488,6 +531,26 @@ __global__ void __launch_bounds__(SkCfg<BN, BK, S, SA, NI>::kThreads, 1)
                 tc::tc_fence_after();
                 const unsigned char* wst = sW8 + st.idx * C::kW8Bytes;
                 const uint32_t a_col = tmem + t_lane + C::kACol + sa.idx * C::kACols;
+                if constexpr (WB == 4) {
+                    // 64 weights (two 16-byte pieces) of this row -> 32 packed half2 -> 32 TMEM columns
+#pragma unroll
+                    for (int c = 0; c < BK / 64; c++) {
+                        constexpr int kPieces = C::kWBoxW / 16;
+                        uint32_t hh[32];
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            const int piece = 2 * c + j;
+                            const uint4 v = *reinterpret_cast<const uint4*>(
+                                wst + piece / kPieces * C::kWBoxBytes + wchunk<C::kWBoxW>(r, piece % kPieces));
+                            const uint32_t s2 = gsv[piece] * 0x10001u;
+                            q4x8_to_h2x4(v.x, s2, hh + 16 * j);
+                            q4x8_to_h2x4(v.y, s2, hh + 16 * j + 4);
+                            q4x8_to_h2x4(v.z, s2, hh + 16 * j + 8);
+                            q4x8_to_h2x4(v.w, s2, hh + 16 * j + 12);
+                        }
+                        tc::tmem_st_32x32b_x32(a_col + c * 32, hh);
+                    }
+                } else
 #pragma unroll
                 for (int h = 0; h < C::kWBoxes; h++) {
                     // 64 int8 of this row -> 32 packed half2 -> 32 TMEM columns
@@ -769,20 +832,23 @@ __global__ void __launch_bounds__(SkCfg<BN, BK, S, SA, NI>::kThreads, 1)
 }
 
 // ----------------------------------------------------------------------------- host
-// Weight map: int8 [N, K] in [128 rows x min(BK, 128) B] boxes (128- or 64-byte
-// swizzle); activation map: fp16 [M, K] in [BN rows x 64] boxes, 128-byte
+// Weight map: int8 [N, K] (or 4-bit, half the bytes) in [128 rows x min(stage row, 128) B] boxes (128-,
+// 64- or 32-byte swizzle); activation map: fp16 [M, K] in [BN rows x 64] boxes, 128-byte
 // swizzled; out-of-range rows/columns read 0.
-bool make_maps(const LinearArgs& a, int BN, int BK, CUtensorMap* mw, CUtensorMap* mx)
+bool make_maps(const LinearArgs& a, int BN, int BK, int wbits, CUtensorMap* mw, CUtensorMap* mx)
 {
+    const int row = BK * wbits / 8;
     TmapDesc w{};
     w.base = a.w;
-    w.inner = a.K;
+    w.inner = a.K * wbits / 8;
     w.outer = a.N;
-    w.row_bytes = a.K;
-    w.box_inner = BK < 128 ? (uint32_t)BK : 128u;
+    w.row_bytes = a.K * wbits / 8;
+    w.box_inner = row < 128 ? (uint32_t)row : 128u;
     w.box_outer = kTileRows;
     w.dtype = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-    w.swizzle = w.box_inner == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    w.swizzle = w.box_inner == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                : w.box_inner == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                    : CU_TENSOR_MAP_SWIZZLE_32B;
     TmapDesc x{};
     x.base = a.x;
     x.inner = a.K;
@@ -862,12 +928,12 @@ long long pick_grid(long long tiles, long long kbpt, int BN, int BK, int num_sms
     return (aligned > tiles && 10 * aligned >= 9 * sk) ? aligned : sk;
 }
 
-template <int BN, int BK, int S, int SA, int NI, typename OT>
-cudaError_t launch_cfg(const LinearArgs& a, int num_sms, const TcScratch& scratch, cudaStream_t stream)
+template <int BN, int BK, int S, int SA, int NI, int WB, typename OT>
+cudaError_t launch_cfg(const LinearArgs& a, const Q4Scales& q, int num_sms, const TcScratch& scratch, cudaStream_t stream)
 {
-    using C = SkCfg<BN, BK, S, SA, NI>;
+    using C = SkCfg<BN, BK, S, SA, NI, WB>;
     CUtensorMap mw, mx, mo;
-    if (!make_maps(a, BN, BK, &mw, &mx)) return cudaErrorInvalidValue;
+    if (!make_maps(a, BN, BK, WB, &mw, &mx)) return cudaErrorInvalidValue;
     const size_t ob = a.out_dtype == kF16 ? 2 : 4;
     const bool tma_out = ((uintptr_t)a.out % 16) == 0 && (a.N * ob) % 16 == 0;
     if (tma_out) {
@@ -875,7 +941,7 @@ cudaError_t launch_cfg(const LinearArgs& a, int num_sms, const TcScratch& scratc
     } else {
         mo = mx;  // unused by the kernel
     }
-    auto kern = q8_gemm_sk_kernel<BN, BK, S, SA, NI, OT>;
+    auto kern = q8_gemm_sk_kernel<BN, BK, S, SA, NI, WB, OT>;
     static thread_local bool configured[64] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -903,6 +969,10 @@ cudaError_t launch_cfg(const LinearArgs& a, int num_sms, const TcScratch& scratc
     // weight stages requested into L2 ahead of the ring measured slower at M = 64: 7B lm_head
     // 146 -> 150-156 us for 8-32 stages ahead.)
     p.w_evict_first = a.M <= (size_t)BN ? 1 : 0;
+    p.gs = q.gs;
+    p.gs_ld = q.ld;
+    p.group_log2 = q.group_log2;
+    p.groups = q.groups;
     const int G = (int)pick_grid(tiles, p.kbpt, BN, BK, num_sms);
     if ((long long)scratch.ws_floats < 2LL * G * BN * kTileRows || (long long)scratch.counters < tiles)
         return cudaErrorMemoryAllocation;
@@ -923,8 +993,8 @@ cudaError_t launch_cfg(const LinearArgs& a, int num_sms, const TcScratch& scratc
     return e;
 }
 
-template <typename OT>
-cudaError_t launch_typed(const LinearArgs& a, int num_sms, const TcScratch& scratch, cudaStream_t stream)
+template <int WB, typename OT>
+cudaError_t launch_typed(const LinearArgs& a, const Q4Scales& q, int num_sms, const TcScratch& scratch, cudaStream_t stream)
 {
     // One A stage in TMEM per shared-memory stage (one commit per stage).  Measured on B200 against
     // the earlier layouts with fewer A stages (16: 5/2, 32: 4/2, 64: 6/3, 128: 4/3 stages), 7B
@@ -936,11 +1006,11 @@ cudaError_t launch_typed(const LinearArgs& a, int num_sms, const TcScratch& scra
     // measured within +-4 %, mostly slower, on the 7B projections and on the config-4 GEMMs at
     // M = 512 (set of four 54.5 vs 54.7 us).
     switch (pick_bn(a.M, a.N, num_sms)) {
-        case 16: return launch_cfg<16, 256, 3, 3, 1, OT>(a, num_sms, scratch, stream);
-        case 32: return launch_cfg<32, 256, 3, 3, 1, OT>(a, num_sms, scratch, stream);
-        case 64: return launch_cfg<64, 128, 6, 6, 2, OT>(a, num_sms, scratch, stream);
-        case 128: return launch_cfg<128, 128, 4, 4, 1, OT>(a, num_sms, scratch, stream);
-        default: return launch_cfg<256, 64, 4, 4, 1, OT>(a, num_sms, scratch, stream);
+        case 16: return launch_cfg<16, 256, 3, 3, 1, WB, OT>(a, q, num_sms, scratch, stream);
+        case 32: return launch_cfg<32, 256, 3, 3, 1, WB, OT>(a, q, num_sms, scratch, stream);
+        case 64: return launch_cfg<64, 128, 6, 6, 2, WB, OT>(a, q, num_sms, scratch, stream);
+        case 128: return launch_cfg<128, 128, 4, 4, 1, WB, OT>(a, q, num_sms, scratch, stream);
+        default: return launch_cfg<256, 64, 4, 4, 1, WB, OT>(a, q, num_sms, scratch, stream);
     }
 }
 
@@ -967,8 +1037,118 @@ void gemm_tc_scratch_need(const LinearArgs& a, int num_sms, size_t* ws_floats, s
 cudaError_t launch_q8_gemm_tc(const LinearArgs& a, int num_sms, const TcScratch& scratch, cudaStream_t stream)
 {
     if (!gemm_tc_supports(a)) return cudaErrorNotSupported;
-    return a.out_dtype == kF16 ? launch_typed<__half>(a, num_sms, scratch, stream)
-                               : launch_typed<float>(a, num_sms, scratch, stream);
+    return a.out_dtype == kF16 ? launch_typed<8, __half>(a, Q4Scales{}, num_sms, scratch, stream)
+                               : launch_typed<8, float>(a, Q4Scales{}, num_sms, scratch, stream);
+}
+
+// ----------------------------------------------------------------------------- 4-bit weights
+namespace {
+
+// Per row: 2^e the power of two at most its largest scale; gs[group][row] = scale * 2^(12 - e) in fp16 (exact down to
+// 2^-29 of that scale; 8 * gs stays below 65504) and row_scale[row] = 2^(e - 12).  Rows up to ld, the tiles'
+// end, are zeros.  A block takes 32 rows: warps read along the rows, and write 32 rows of a group at a time.
+// Bound by HBM and its launch (2 bytes read and written per group).
+__global__ void __launch_bounds__(256) q4_scale_prep_kernel(const uint16_t* __restrict__ scales, __half* __restrict__ gs,
+                                                            float* __restrict__ row_scale, int N, int ng, int ld)
+{
+    __shared__ int row_e[32];
+    __shared__ uint16_t tile[32][65];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row0 = blockIdx.x * 32;
+    pdl_wait();
+    // Only now may the GEMM start: it reads weights before it waits for this kernel, and what wrote
+    // them is complete from here on.
+    pdl_launch_dependents();
+    for (int r = warp; r < 32; r += 8) {
+        const int n = row0 + r;
+        int top = 0;
+        if (n < N)
+            for (int j = lane; j < ng; j += 32) top = max(top, scales[(size_t)n * ng + j] & 0x7FFF);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int e = top == 0 ? 0 : max((top >> 7) - 127, -126);  // subnormal scales count as 2^-126
+        if (lane == 0) {
+            row_e[r] = e;
+            if (n < N) row_scale[n] = ldexpf(1.0f, e - 12);
+        }
+    }
+    __syncthreads();
+    for (int g0 = 0; g0 < ng; g0 += 64) {
+        const int cnt = min(64, ng - g0);
+        for (int r = warp; r < 32; r += 8) {
+            const int n = row0 + r;
+            for (int j = lane; j < cnt; j += 32) {
+                const float s = n < N ? __uint_as_float((uint32_t)scales[(size_t)n * ng + g0 + j] << 16) : 0.0f;
+                tile[r][j] = __half_as_ushort(__float2half_rn(ldexpf(s, 12 - row_e[r])));
+            }
+        }
+        __syncthreads();
+        for (int j = warp; j < cnt; j += 8)
+            gs[(size_t)(g0 + j) * ld + row0 + lane] = __ushort_as_half(tile[lane][j]);
+        __syncthreads();
+    }
+}
+
+LinearArgs as_linear(const Q4Args& a)
+{
+    LinearArgs l;
+    l.x = a.x;
+    l.w = reinterpret_cast<const int8_t*>(a.q4);
+    l.bias = a.bias;
+    l.res = a.res;
+    l.out = a.out;
+    l.M = a.M;
+    l.N = a.N;
+    l.K = a.K;
+    l.in_dtype = a.in_dtype;
+    l.out_dtype = a.out_dtype;
+    l.pdl = true;
+    return l;
+}
+
+}  // namespace
+
+bool q4_gemm_tc_supports(const Q4Args& a)
+{
+    return a.K % 32 == 0 && a.N <= (size_t)INT32_MAX - 128 && gemm_tc_supports(as_linear(a));
+}
+
+void q4_gemm_tc_scratch_need(const Q4Args& a, int num_sms, size_t* ws_floats, size_t* counters, size_t* act_bytes)
+{
+    gemm_tc_scratch_need(as_linear(a), num_sms, ws_floats, counters);
+    const size_t ld = (a.N + kTileRows - 1) / kTileRows * kTileRows;
+    *act_bytes = ld * 4 + ld * ((a.K + a.group - 1) / a.group) * 2;
+}
+
+cudaError_t launch_q4_gemm_tc(const Q4Args& a, int num_sms, const TcScratch& scratch, cudaStream_t stream)
+{
+    if (!q4_gemm_tc_supports(a)) return cudaErrorNotSupported;
+    size_t ws = 0, counters = 0, act = 0;
+    q4_gemm_tc_scratch_need(a, num_sms, &ws, &counters, &act);
+    if (scratch.act_bytes < act) return cudaErrorMemoryAllocation;
+    Q4Scales q;
+    q.ld = (int)((a.N + kTileRows - 1) / kTileRows * kTileRows);
+    q.group_log2 = a.group == 32 ? 5 : a.group == 64 ? 6 : 7;
+    q.groups = (int)((a.K + a.group - 1) / a.group);
+    float* row_scale = reinterpret_cast<float*>(scratch.act);
+    __half* gs = reinterpret_cast<__half*>(row_scale + q.ld);
+    q.gs = gs;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(q.ld / 32));
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, q4_scale_prep_kernel, a.scales, gs, row_scale, (int)a.N, q.groups, q.ld);
+    if (e != cudaSuccess) return e;
+    note_launch();
+    LinearArgs l = as_linear(a);
+    l.scales = row_scale;
+    return a.out_dtype == kF16 ? launch_typed<4, __half>(l, q, num_sms, scratch, stream)
+                               : launch_typed<4, float>(l, q, num_sms, scratch, stream);
 }
 
 #ifdef B200Q8_TRACE
