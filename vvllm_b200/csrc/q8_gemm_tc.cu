@@ -507,19 +507,28 @@ __global__ void __launch_bounds__(SkCfg<BN, BK, S, SA, NI, WB>::kThreads, 1)
         bool ok = true;
         long long w_full = 0, w_aempty = 0;
         const long long t_role = clock64();
+        // 4-bit weights: this row's scale of every 32 weights of this warp's next stage (a group is one, two or
+        // four times 32; behind K the weights meet zero activations)
+        uint32_t gs_next[WB == 4 ? BK / 32 : 1];
+        auto load_gs = [&](int tile, int kb) {
+            if constexpr (WB == 4) {
+                const __half* gp = p.gs + (tile % p.tiles_n) * kTileRows + r;
+#pragma unroll
+                for (int c = 0; c < BK / 32; c++) {
+                    const int gi = min((kb * BK + c * 32) >> p.group_log2, p.groups - 1);
+                    gs_next[c] = __half_as_ushort(__ldg(gp + (size_t)gi * p.gs_ld));
+                }
+            }
+        };
         while (ok && it.next(t, k0, k1)) {
             for (int kb = k0; kb < k1; kb++, g++, st.next(S), sa.next(SA)) {
                 if ((g & 1) != group) continue;
-                // 4-bit weights: this row's scale of every 32 weights of the stage (a group is one, two or four
-                // times 32; behind K the weights meet zero activations)
                 uint32_t gsv[WB == 4 ? BK / 32 : 1];
                 if constexpr (WB == 4) {
-                    const __half* gp = p.gs + (t % p.tiles_n) * kTileRows + r;
+                    if (kb - k0 < 2) load_gs(t, kb);  // this warp's first stage of the segment
 #pragma unroll
-                    for (int c = 0; c < BK / 32; c++) {
-                        const int gi = min((kb * BK + c * 32) >> p.group_log2, p.groups - 1);
-                        gsv[c] = __half_as_ushort(__ldg(gp + (size_t)gi * p.gs_ld));
-                    }
+                    for (int c = 0; c < BK / 32; c++) gsv[c] = gs_next[c] * 0x10001u;
+                    if (kb + 2 < k1) load_gs(t, kb + 2);
                 }
                 ok = __all_sync(0xffffffffu, timed_wait(full0 + 8u * st.idx, st.phase, abort, w_full));
                 if (!ok) break;
@@ -542,7 +551,7 @@ __global__ void __launch_bounds__(SkCfg<BN, BK, S, SA, NI, WB>::kThreads, 1)
                             const int piece = 2 * c + j;
                             const uint4 v = *reinterpret_cast<const uint4*>(
                                 wst + piece / kPieces * C::kWBoxBytes + wchunk<C::kWBoxW>(r, piece % kPieces));
-                            const uint32_t s2 = gsv[piece] * 0x10001u;
+                            const uint32_t s2 = gsv[piece];
                             q4x8_to_h2x4(v.x, s2, hh + 16 * j);
                             q4x8_to_h2x4(v.y, s2, hh + 16 * j + 4);
                             q4x8_to_h2x4(v.z, s2, hh + 16 * j + 8);
@@ -1046,45 +1055,50 @@ namespace {
 
 // Per row: 2^e the power of two at most its largest scale; gs[group][row] = scale * 2^(12 - e) in fp16 (exact down to
 // 2^-29 of that scale; 8 * gs stays below 65504) and row_scale[row] = 2^(e - 12).  Rows up to ld, the tiles'
-// end, are zeros.  A block takes 32 rows: warps read along the rows, and write 32 rows of a group at a time.
-// Bound by HBM and its launch (2 bytes read and written per group).
+// end, are zeros.  A block takes 32 rows, eight threads a row; up to 160 groups at a time are in registers
+// (rows of more are read twice) and go through shared memory to be written 32 rows of a group at a time.
+// Bound by its launch and one round of memory latency (2 bytes read and written per group).
+constexpr int kPrepGroups = 160;
 __global__ void __launch_bounds__(256) q4_scale_prep_kernel(const uint16_t* __restrict__ scales, __half* __restrict__ gs,
                                                             float* __restrict__ row_scale, int N, int ng, int ld)
 {
-    __shared__ int row_e[32];
-    __shared__ uint16_t tile[32][65];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row0 = blockIdx.x * 32;
+    constexpr int V = kPrepGroups / 8;
+    __shared__ uint16_t tile[32][kPrepGroups + 2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = threadIdx.x >> 3, l = threadIdx.x & 7;
+    const int row0 = blockIdx.x * 32, n = row0 + r;
     pdl_wait();
     // Only now may the GEMM start: it reads weights before it waits for this kernel, and what wrote
     // them is complete from here on.
     pdl_launch_dependents();
-    for (int r = warp; r < 32; r += 8) {
-        const int n = row0 + r;
-        int top = 0;
-        if (n < N)
-            for (int j = lane; j < ng; j += 32) top = max(top, scales[(size_t)n * ng + j] & 0x7FFF);
+    const uint16_t* src = scales + (size_t)min(n, N - 1) * ng;
+    uint32_t v[V];
+    auto load = [&](int g0) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int e = top == 0 ? 0 : max((top >> 7) - 127, -126);  // subnormal scales count as 2^-126
-        if (lane == 0) {
-            row_e[r] = e;
-            if (n < N) row_scale[n] = ldexpf(1.0f, e - 12);
+        for (int i = 0; i < V; i++) {
+            const int j = g0 + l + 8 * i;
+            v[i] = n < N && j < ng ? src[j] : 0u;
         }
+    };
+    uint32_t top = 0;
+    for (int g0 = (ng - 1) / kPrepGroups * kPrepGroups; g0 >= 0; g0 -= kPrepGroups) {  // ends with the first groups
+        load(g0);
+#pragma unroll
+        for (int i = 0; i < V; i++) top = max(top, v[i] & 0x7FFFu);
     }
-    __syncthreads();
-    for (int g0 = 0; g0 < ng; g0 += 64) {
-        const int cnt = min(64, ng - g0);
-        for (int r = warp; r < 32; r += 8) {
-            const int n = row0 + r;
-            for (int j = lane; j < cnt; j += 32) {
-                const float s = n < N ? __uint_as_float((uint32_t)scales[(size_t)n * ng + g0 + j] << 16) : 0.0f;
-                tile[r][j] = __half_as_ushort(__float2half_rn(ldexpf(s, 12 - row_e[r])));
-            }
-        }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int e = top == 0 ? 0 : max((int)(top >> 7) - 127, -126);  // subnormal scales count as 2^-126
+    if (l == 0 && n < N) row_scale[n] = ldexpf(1.0f, e - 12);
+    const int up = 12 - e;  // -116 .. 138: in two exact factors
+    const float f0 = __uint_as_float((uint32_t)(up / 2 + 127) << 23), f1 = __uint_as_float((uint32_t)(up - up / 2 + 127) << 23);
+    for (int g0 = 0; g0 < ng; g0 += kPrepGroups) {
+        const int cnt = min(kPrepGroups, ng - g0);
+        if (g0) load(g0);
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            tile[r][l + 8 * i] = __half_as_ushort(__float2half_rn(__uint_as_float(v[i] << 16) * f0 * f1));
         __syncthreads();
-        for (int j = warp; j < cnt; j += 8)
-            gs[(size_t)(g0 + j) * ld + row0 + lane] = __ushort_as_half(tile[lane][j]);
+        for (int j = warp; j < cnt; j += 8) gs[(size_t)(g0 + j) * ld + row0 + lane] = __ushort_as_half(tile[lane][j]);
         __syncthreads();
     }
 }
