@@ -206,7 +206,7 @@ struct LogitArgs {
     const uint32_t* allowed = nullptr;  // [M] rows of allowed_stride words, bit i % 32 of word i / 32; or null
     size_t allowed_stride = 0;
 };
-cudaError_t launch_logits(const LogitArgs& a, size_t max_smem, cudaStream_t stream);
+cudaError_t launch_logits(const LogitArgs& a, int num_sms, size_t max_smem, cudaStream_t stream);
 
 // Reads (and optionally clears) the device error word the tensor-core kernel
 // sets when a bounded wait gives up (bit 0).

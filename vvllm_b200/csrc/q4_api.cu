@@ -258,7 +258,7 @@ int b200q8_process_logits(void* out, int out_dtype, size_t out_stride, const voi
     a.bias_count = r.bias_count;
     a.allowed = r.allowed;
     a.allowed_stride = r.allowed_stride;
-    cudaError_t e = launch_logits(a, smem, (cudaStream_t)stream);
+    cudaError_t e = launch_logits(a, sms, smem, (cudaStream_t)stream);
     return e == cudaSuccess ? B200Q8_OK : cuda_fail(e, "process_logits launch");
 }
 
