@@ -248,45 +248,57 @@ def quantize_per_channel_bf16(w_bits, q, scales, stream=None) -> None:
     _check(lib().b200q8_quantize_per_channel_bf16(_addr(w_bits), N, K, _addr(q), _addr(scales), _stream(stream)))
 
 
-def _same_device(name: str, *tensors) -> None:
-    """Every tensor given lies on the current CUDA device (kernels run there, on raw addresses)."""
-    import torch
+_torch = None
 
-    dev = -1
-    for t in tensors:
-        if t is None:
-            continue
-        d = t.get_device()
-        if d < 0:
-            raise ValueError(f"{name}: CUDA tensors only, got one on {t.device}")
-        if dev < 0:
-            dev = torch.cuda.current_device()
-        if d != dev:
-            raise ValueError(f"{name}: a tensor lies on cuda:{d}, the current device is cuda:{dev}")
+
+def _t():
+    """The torch module, imported with the first call that needs its types."""
+    global _torch
+    if _torch is None:
+        import torch
+
+        _torch = torch
+    return _torch
+
+
+def _same_device(name: str, first, *others) -> None:
+    """Every tensor given lies on the current CUDA device (kernels run there, on raw addresses)."""
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name}: tensors on {first.device} and {t.device}")
+    if dev < 0:
+        raise ValueError(f"{name}: CUDA tensors only, got one on {first.device}")
+    if dev != _torch.cuda.current_device():
+        raise ValueError(f"{name}: the tensors lie on cuda:{dev}, the current device is cuda:{_torch.cuda.current_device()}")
 
 
 def _expect(name: str, what: str, t, shape: tuple, dtype) -> None:
     """t is a contiguous tensor of that shape and type."""
-    if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
+    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous():
         raise ValueError(f"{name}: {what} must be contiguous {list(shape)} of {dtype}, got {list(t.shape)} of {t.dtype}")
 
 
 def _expect_q4(name: str, q4, scales, group: int, N: int, K: int) -> None:
-    import torch
-
     if group not in (32, 64, 128):
         raise ValueError(f"{name}: group must be 32, 64 or 128, got {group}")
-    _expect(name, "q4", q4, (N, (K + 1) // 2), torch.uint8)
-    _expect(name, "scales", scales, (N, -(-K // group)), torch.bfloat16)
+    _expect(name, "q4", q4, (N, (K + 1) // 2), _torch.uint8)
+    _expect(name, "scales", scales, (N, -(-K // group)), _torch.bfloat16)
+
+
+def _float_code(name: str, what: str, t) -> int:
+    if t.dtype is _torch.float16:
+        return F16
+    if t.dtype is _torch.float32:
+        return F32
+    raise ValueError(f"{name}: {what} must be fp32 or fp16, got {t.dtype}")
 
 
 def quantize_q4(w, q4, scales, group: int, stream=None) -> None:
     """q4[N,ceil(K/2)] uint8, scales[N,ceil(K/group)] bf16 = 4-bit group quantization of w[N,K] fp32
     (element 2j in the low, 2j+1 in the high half of byte j, as q + 8; value q * scale)."""
-    import torch
-
     N, K = w.shape
-    _expect("quantize_q4", "w", w, (N, K), torch.float32)
+    _expect("quantize_q4", "w", w, (N, K), _t().float32)
     _expect_q4("quantize_q4", q4, scales, group, N, K)
     _same_device("quantize_q4", w, q4, scales)
     _check(lib().b200q8_quantize_q4(w.data_ptr(), N, K, group, q4.data_ptr(), scales.data_ptr(), _stream(stream)))
@@ -294,10 +306,9 @@ def quantize_q4(w, q4, scales, group: int, stream=None) -> None:
 
 def quantize_q4_bf16(w, q4, scales, group: int, stream=None) -> None:
     """The same from w[N,K] bfloat16 (or its bits as int16 / uint16)."""
-    import torch
-
     N, K = w.shape
-    _expect("quantize_q4_bf16", "w", w, (N, K), w.dtype if w.dtype in (torch.int16, torch.uint16) else torch.bfloat16)
+    bits = (_t().int16, _t().uint16)
+    _expect("quantize_q4_bf16", "w", w, (N, K), w.dtype if w.dtype in bits else _torch.bfloat16)
     _expect_q4("quantize_q4_bf16", q4, scales, group, N, K)
     _same_device("quantize_q4_bf16", w, q4, scales)
     _check(lib().b200q8_quantize_q4_bf16(w.data_ptr(), N, K, group, q4.data_ptr(), scales.data_ptr(), _stream(stream)))
@@ -306,16 +317,18 @@ def quantize_q4_bf16(w, q4, scales, group: int, stream=None) -> None:
 def dequantize_q4(out, q4, scales, group: int, rows=None, stream=None) -> None:
     """out[R,K] (fp32 or fp16) = values of the rows rows[R] (int32; an index outside the matrix gives
     zeros: the token lookup of a 4-bit embedding), or of all rows."""
-    import torch
-
     N, (R, K) = q4.shape[0], out.shape
+    _t()
     _expect_q4("dequantize_q4", q4, scales, group, N, K)
     _expect("dequantize_q4", "out", out, (R if rows is not None else N, K), out.dtype)
+    code, at = _float_code("dequantize_q4", "out", out), None
     if rows is not None:
-        _expect("dequantize_q4", "rows", rows, (R,), torch.int32)
+        _expect("dequantize_q4", "rows", rows, (R,), _torch.int32)
+        at = rows.data_ptr()
     _same_device("dequantize_q4", out, q4, scales, rows)
-    _check(lib().b200q8_dequantize_q4(out.data_ptr(), _dtype_code(out), q4.data_ptr(), scales.data_ptr(), group,
-                                      _addr(rows), R, N, K, _stream(stream)))
+    if R:  # (no rows: an empty list has no address)
+        _check(lib().b200q8_dequantize_q4(out.data_ptr(), code, q4.data_ptr(), scales.data_ptr(), group, at, R, N, K,
+                                          _stream(stream)))
 
 
 def linear_q4(out, x, q4, scales, group: int, bias=None, stream=None) -> None:
@@ -325,21 +338,24 @@ def linear_q4(out, x, q4, scales, group: int, bias=None, stream=None) -> None:
 
 def linear_q4_add(out, x, q4, scales, group: int, bias, residual, stream=None) -> None:
     """The same plus residual[M,N] (out's type; may be out itself), added last."""
-    import torch
-
+    name = "linear_q4"
     M, K = x.shape
     N = q4.shape[0]
-    _expect_q4("linear_q4", q4, scales, group, N, K)
-    _expect("linear_q4", "x", x, (M, K), x.dtype)
-    _expect("linear_q4", "out", out, (M, N), out.dtype)
+    _t()
+    _expect_q4(name, q4, scales, group, N, K)
+    _expect(name, "x", x, (M, K), x.dtype)
+    _expect(name, "out", out, (M, N), out.dtype)
+    b = r = None
     if bias is not None:
-        _expect("linear_q4", "bias", bias, (N,), torch.float32)
+        _expect(name, "bias", bias, (N,), _torch.float32)
+        b = bias.data_ptr()
     if residual is not None:
-        _expect("linear_q4", "residual", residual, (M, N), out.dtype)
-    _same_device("linear_q4", x, out, q4, scales, bias, residual)
-    _check(lib().b200q8_linear_q4_add(out.data_ptr(), _dtype_code(out), x.data_ptr(), _dtype_code(x), q4.data_ptr(),
-                                      scales.data_ptr(), group, _addr(bias), _addr(residual), M, N, K,
-                                      _stream(stream)))
+        _expect(name, "residual", residual, (M, N), out.dtype)
+        r = residual.data_ptr()
+    ocode, xcode = _float_code(name, "out", out), _float_code(name, "x", x)
+    _same_device(name, x, out, q4, scales, bias, residual)
+    _check(lib().b200q8_linear_q4_add(out.data_ptr(), ocode, x.data_ptr(), xcode, q4.data_ptr(), scales.data_ptr(), group,
+                                      b, r, M, N, K, _stream(stream)))
 
 
 class _LogitRules(ctypes.Structure):
@@ -349,17 +365,24 @@ class _LogitRules(ctypes.Structure):
                 ("allowed_stride", _sz)]
 
 
-def _row_stride(name: str, what: str, t, M: int) -> int:
-    """Row stride of t: [M, n] with contiguous rows, or [n] / [1, n] shared by all rows (0)."""
-    if t.dim() == 1:
-        t = t.unsqueeze(0)
-    if t.dim() != 2 or t.shape[0] not in (1, M) or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name}: {what} must be [M, n] with contiguous rows, or one such row for all")
-    if t.shape[0] == 1 or t.stride(0) == 0:
-        return 0
-    if t.stride(0) < t.shape[1]:
+def _rows_of(name: str, what: str, t, M: int, dtype):
+    """(address, row stride, columns) of t: [M, n] with contiguous rows, or [n] / [1, n] shared by all rows
+    (stride 0).  No columns: no address."""
+    shape, n = t.shape, t.shape[-1] if t.dim() else 0
+    if t.dtype is not dtype or not (len(shape) == 2 and shape[0] in (1, M) or len(shape) == 1) or (n > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name}: {what} must be [M, n] {dtype} with contiguous rows, or one such row for all, "
+                         f"got {list(shape)} of {t.dtype}")
+    stride = t.stride(0) if len(shape) == 2 and shape[0] > 1 else 0
+    if 0 < stride < n:
         raise ValueError(f"{name}: rows of {what} overlap")
-    return t.stride(0)
+    return t.data_ptr() or None, stride, n
+
+
+def _per_row(name: str, what: str, t, M: int, dtype):
+    if t is None:
+        return None
+    _expect(name, what, t, (M,), dtype)
+    return t.data_ptr()
 
 
 def process_logits(out, logits, argmax=None, history=None, history_len=None, prompt_len=None, repetition=None,
@@ -371,47 +394,43 @@ def process_logits(out, logits, argmax=None, history=None, history_len=None, pro
     out: fp32 or fp16, logits itself, or None.  history / bias_ids / bias_values / allowed: [M, n]
     int32 / int32 / fp32 / int32 (bit i % 32 of word i // 32), or one row for all; the other rules are
     [M]: int32 lengths and fp32 penalties.  Rows of every 2-D tensor are contiguous, any row stride."""
-    import torch
-
     name = "process_logits"
     M, V = logits.shape
-    if logits.stride(1) != 1 and V > 1 or (out is not None and (tuple(out.shape) != (M, V)
-                                                                or (out.stride(1) != 1 and V > 1))):
+    i32, f32 = _t().int32, _torch.float32
+    if V > 1 and (logits.stride(1) != 1 or (out is not None and out.stride(-1) != 1)) or (
+            out is not None and out.shape != (M, V)):
         raise ValueError(f"{name}: logits and out must be [{M}, {V}] with contiguous rows")
-    r = _LogitRules()
-    i32, f32 = torch.int32, torch.float32
-    for what, t, dt in (("argmax", argmax, i32), ("history_len", history_len, i32), ("prompt_len", prompt_len, i32),
-                        ("repetition", repetition, f32), ("presence", presence, f32), ("frequency", frequency, f32),
-                        ("bias_len", bias_len, i32)):
-        if t is not None:
-            _expect(name, what, t, (M,), dt)
-            if what != "argmax":
-                setattr(r, what, t.data_ptr())
-    for what, t, dt in (("history", history, i32), ("bias_ids", bias_ids, i32), ("bias_values", bias_values, f32),
-                        ("allowed", allowed, i32)):
-        if t is not None:
-            if t.dtype != dt:
-                raise ValueError(f"{name}: {what} must be {dt}, got {t.dtype}")
-            stride = _row_stride(name, what, t, M)
-            setattr(r, what, t.data_ptr())
-            if what == "history":
-                r.history_stride, r.history_count = stride, t.shape[-1]
-            elif what == "bias_ids":
-                r.bias_stride, r.bias_count = stride, t.shape[-1]
-            elif what == "bias_values":
-                if bias_ids is None or t.shape[-1] != bias_ids.shape[-1] or stride != r.bias_stride:
-                    raise ValueError(f"{name}: bias_values must be laid out like bias_ids")
-            else:
-                if t.shape[-1] < (V + 31) // 32:
-                    raise ValueError(f"{name}: allowed needs {(V + 31) // 32} words a row, got {t.shape[-1]}")
-                r.allowed_stride = stride
+    am = _per_row(name, "argmax", argmax, M, i32)
+    rules = None
+    hist = bids = bvals = mask = None
+    if history is not None or bias_ids is not None or bias_values is not None or allowed is not None:
+        hstride = hcount = bstride = bcount = mstride = 0
+        if history is not None:
+            hist, hstride, hcount = _rows_of(name, "history", history, M, i32)
+        if bias_ids is not None:
+            bids, bstride, bcount = _rows_of(name, "bias_ids", bias_ids, M, i32)
+        if bias_values is not None:
+            bvals, vstride, vcount = _rows_of(name, "bias_values", bias_values, M, f32)
+            if bias_ids is None or (vstride, vcount) != (bstride, bcount):
+                raise ValueError(f"{name}: bias_values must be laid out like bias_ids")
+        if allowed is not None:
+            mask, mstride, words = _rows_of(name, "allowed", allowed, M, i32)
+            if words < (V + 31) // 32:
+                raise ValueError(f"{name}: allowed needs {(V + 31) // 32} words a row, got {words}")
+        rules = _LogitRules(hist, hstride, hcount, _per_row(name, "history_len", history_len, M, i32),
+                            _per_row(name, "prompt_len", prompt_len, M, i32),
+                            _per_row(name, "repetition", repetition, M, f32), _per_row(name, "presence", presence, M, f32),
+                            _per_row(name, "frequency", frequency, M, f32), bids, bvals, bstride, bcount,
+                            _per_row(name, "bias_len", bias_len, M, i32), mask, mstride)
     _same_device(name, logits, out, argmax, history, history_len, prompt_len, repetition, presence, frequency, bias_ids,
                  bias_values, bias_len, allowed)
-    in_stride = logits.stride(0) if M > 1 else V
-    out_stride = V if out is None or M == 1 else out.stride(0)
-    _check(lib().b200q8_process_logits(_addr(out), _dtype_code(logits if out is None else out), out_stride,
-                                       logits.data_ptr(), _dtype_code(logits), in_stride, M, V, ctypes.byref(r),
-                                       _addr(argmax), _stream(stream)))
+    xcode = _float_code(name, "logits", logits)
+    if out is None:
+        to, ocode, ostride = None, xcode, V
+    else:
+        to, ocode, ostride = out.data_ptr(), _float_code(name, "out", out), out.stride(0) if M > 1 else V
+    _check(lib().b200q8_process_logits(to, ocode, ostride, logits.data_ptr(), xcode, logits.stride(0) if M > 1 else V, M, V,
+                                       None if rules is None else ctypes.addressof(rules), am, _stream(stream)))
 
 
 ST_F32, ST_F16, ST_BF16, ST_I8, ST_OTHER = 0, 1, 2, 3, 4
