@@ -179,6 +179,12 @@ __device__ __forceinline__ void mma16832(int (&d)[4], int start, uint32_t a0, ui
 constexpr int kMagicBits = 0x4B400000;
 constexpr float kMagic = 12582912.0f;
 
+// The sums of a fragment's columns 2t and 2t + 1 in row `i`.
+__device__ __forceinline__ float2 tile_value(const int (&d)[4], int i)
+{
+    return __fadd2_rn(make_float2(__int_as_float(d[2 * i]), __int_as_float(d[2 * i + 1])), make_float2(-kMagic, -kMagic));
+}
+
 // Shared memory distance of two columns of `blocks` 32-blocks of bytes, two blocks to 64 bytes: an odd
 // number of those, so that neighbouring columns' loads fall into different banks.
 __host__ __device__ constexpr size_t column_stride(int blocks) { return (size_t)((blocks / 2) | 1) * 64; }
@@ -195,7 +201,7 @@ __device__ __forceinline__ int column_of(int m, int d, int M)  // where it is st
 //   xs      [column][pair of blocks][quarter t][2 blocks] of 8 bytes: the bytes that lane t multiplies
 //           with its word of a block, elements 0 2 4 6 1 3 5 7.  Within a group of W = group / 32 blocks, word
 //           w of lane t starts at element (t * W + w) * 8.  Zero behind K.
-//   weight  [chunk][8 NT]: what a column's integer counts, with the 1/16 of the codes' bytes
+//   weight  [chunk][8]: what a column's integer (NT == 1; else a token's X) counts, with the 1/16 of the codes' bytes
 //   direct  [token][chunk]: 1 if the chunk is summed directly; returns whether this thread saw any
 // Half a warp per chunk of 128 elements, eight elements a lane; a few chunks' loads at a time.  `then` is
 // called once the first loads are under way.
@@ -273,9 +279,8 @@ __device__ __forceinline__ bool stage_tokens(unsigned char* xs, float* weight, u
 #pragma unroll
                 for (int n = 0; n < 3; n++)
                     *reinterpret_cast<uint2*>(dst + column_of<NT>(m, n, p.M) * cs) = make_uint2(d[n][0], d[n][1]);
-                if (u < 3)
-                    weight[c * 8 * NT + (NT == 1 ? 3 * m + u : 8 * u + m)] =
-                        __uint_as_float((uint32_t)(e - 22 - 4 + 8 * u + 127) << 23);
+                if (u < (NT == 1 ? 3 : 1))
+                    weight[c * 8 + (NT == 1 ? 3 * m + u : m)] = __uint_as_float((uint32_t)(e - 22 - 4 + 8 * u + 127) << 23);
                 if (u == 3) direct[m * chunks + c] = bad;
                 any |= bad;
             }
@@ -317,7 +322,7 @@ template <int NT, int IB>
 struct StreamCfg {
     static constexpr int kItemBytes = IB * kBoxBytes;
     static constexpr int kChunks = IB * kBoxK / 128;  // 128-chunks of an item
-    static constexpr int kCols = 8 * NT;              // columns kept in `weight`
+    static constexpr int kCols = 8;                   // columns kept in `weight`: NT == 1 the tile's, else the tokens
     static constexpr int kSums = NT == 1 ? 2 * 16 : 8 * 16;  // a tile's outputs: [token][row]
     static size_t smem(int warps, int stages, int M, int per, int cluster)
     {
@@ -402,27 +407,34 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
             tc::tma_load_2d_hint(ring + stage * kItemBytes + b * kBoxBytes, &tmW, (ich * IB + b) * 128, itile * 16,
                                  bar0 + 8 * stage, policy);
     };
-    // Scales of the chunk about to be multiplied, loaded while the one before is.
-    uint32_t sc0[GC], sc1[GC];
-    const uint16_t *sp0 = nullptr, *sp1 = nullptr;
-    int sg = 0;  // group index that sp0, sp1 point at
+    // Scales of the chunk about to be multiplied, two to a word, loaded while the one before is.
+    constexpr int kSW = (GC + 1) / 2;
+    uint32_t sc0[kSW], sc1[kSW];
+    const uint16_t* sp = nullptr;  // of the fragment's first row; the other row's lie `srow` behind
+    size_t srow = 0;
+    int sg = 0;  // group index that sp points at
+    const bool swide = GC == 4 && ng % 4 == 0 && ((uintptr_t)p.a.scales & 7) == 0;  // four scales in one load
     auto load_scales = [&]() {
-        if (sg + GC <= ng) {
-#pragma unroll
-            for (int i = 0; i < GC; i++) sc0[i] = __ldg(sp0 + i), sc1[i] = __ldg(sp1 + i);
-        } else {  // a row's last item may be short
+        if (GC == 4 && swide) {
+            const uint2 a = sg < ng ? __ldg(reinterpret_cast<const uint2*>(sp)) : make_uint2(0, 0);
+            const uint2 b = sg < ng ? __ldg(reinterpret_cast<const uint2*>(sp + srow)) : make_uint2(0, 0);
+            sc0[0] = a.x, sc1[0] = b.x;
+            if constexpr (kSW == 2) sc0[1] = a.y, sc1[1] = b.y;
+        } else {
 #pragma unroll
             for (int i = 0; i < GC; i++) {
-                const bool in = sg + i < ng;
-                sc0[i] = in ? (uint32_t)__ldg(sp0 + i) : 0u;
-                sc1[i] = in ? (uint32_t)__ldg(sp1 + i) : 0u;
+                const bool in = sg + i < ng;  // a row's last item may be short
+                const uint32_t a = in ? (uint32_t)__ldg(sp + i) : 0u, b = in ? (uint32_t)__ldg(sp + srow + i) : 0u;
+                sc0[i / 2] = i & 1 ? sc0[i / 2] | a << 16 : a;
+                sc1[i / 2] = i & 1 ? sc1[i / 2] | b << 16 : b;
             }
         }
     };
     auto first_scales = [&](int tile) {
+        const int n0 = min(tile * 16 + row, N - 1), n1 = min(tile * 16 + row + 8, N - 1);
         sg = (ch0 + kw) * C::kChunks * GC;
-        sp0 = p.a.scales + (size_t)min(tile * 16 + row, N - 1) * ng + sg;
-        sp1 = p.a.scales + (size_t)min(tile * 16 + row + 8, N - 1) * ng + sg;
+        sp = p.a.scales + (size_t)n0 * ng + sg;
+        srow = (size_t)(n1 - n0) * ng;
         load_scales();
     };
     // The tokens' loads go first and one item a warp behind them, the others once the tokens are done: behind
@@ -457,11 +469,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
         const int tile = tile0 + it * tstep;
         if (tile >= p.tiles) break;  // groups end on their own; with a cluster there is one group
         if (lane == 0 && kw == 0 && tile + tstep < p.tiles) prefetch_scales(tile + tstep);
-        float acc[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[nt][i] = 0.0f;
+        // Of rows row and row + 8: columns 2t and 2t + 1, which are tokens where three tiles hold their bytes.
+        float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
         for (int ch = ch0 + kw; ch < ch1; ch += wk) {
             if (ok) {
                 ok = __all_sync(0xffffffffu, tc::mbar_wait(bar0 + 8 * stage, phase, &zero, kWaitNs));
@@ -476,13 +485,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
             for (int c = 0; c < C::kChunks; c++) {
                 float s0[GC], s1[GC];
 #pragma unroll
-                for (int i = 0; i < GC; i++) s0[i] = bf16_bits_to_f32(sc0[i]), s1[i] = bf16_bits_to_f32(sc1[i]);
-                if (c + 1 < C::kChunks) {
-                    sp0 += GC, sp1 += GC, sg += GC;
-                    load_scales();
-                } else if (ch + wk < ch1) {
-                    const int step = ((wk - 1) * C::kChunks + 1) * GC;
-                    sp0 += step, sp1 += step, sg += step;
+                for (int i = 0; i < GC; i++) {
+                    s0[i] = __uint_as_float(i & 1 ? sc0[i / 2] & 0xFFFF0000u : sc0[i / 2] << 16);
+                    s1[i] = __uint_as_float(i & 1 ? sc1[i / 2] & 0xFFFF0000u : sc1[i / 2] << 16);
+                }
+                if (c + 1 < C::kChunks || ch + wk < ch1) {
+                    const int step = c + 1 < C::kChunks ? GC : ((wk - 1) * C::kChunks + 1) * GC;
+                    sp += step, sg += step;
                     load_scales();
                 } else if (tile + tstep < p.tiles) {
                     first_scales(tile + tstep);
@@ -493,7 +502,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
                     lds<4>(xoff[nt] + xitem, x[nt][0]);
                     lds<4>(xoff[nt] + xitem + 64, x[nt][1]);
                 }
-                float sum[NT][4];
+                float2 sum[2];
 #pragma unroll
                 for (int gi = 0; gi < GC; gi++) {
                     uint32_t w0[W], w1[W];
@@ -516,30 +525,24 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
                         }
                     }
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float f = __int_as_float(d[nt][i]) - kMagic, r = i < 2 ? s0[gi] : s1[gi];
-                            sum[nt][i] = gi == 0 ? f * r : fmaf(f, r, sum[nt][i]);
-                        }
+                    for (int i = 0; i < 2; i++) {
+                        const float r = i == 0 ? s0[gi] : s1[gi];
+                        float2 f = tile_value(d[0], i);
+                        if constexpr (NT == 3)  // X0 + 256 X1 + 65536 X2
+                            f = __ffma2_rn(__ffma2_rn(tile_value(d[2], i), make_float2(256.0f, 256.0f), tile_value(d[1], i)),
+                                           make_float2(256.0f, 256.0f), f);
+                        sum[i] = gi == 0 ? __fmul2_rn(f, make_float2(r, r)) : __ffma2_rn(f, make_float2(r, r), sum[i]);
+                    }
                 }
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    const float2 wt = *reinterpret_cast<const float2*>(wchunk + nt * 8);
-                    acc[nt][0] = fmaf(sum[nt][0], wt.x, acc[nt][0]);
-                    acc[nt][1] = fmaf(sum[nt][1], wt.y, acc[nt][1]);
-                    acc[nt][2] = fmaf(sum[nt][2], wt.x, acc[nt][2]);
-                    acc[nt][3] = fmaf(sum[nt][3], wt.y, acc[nt][3]);
-                }
+                const float2 wt = *reinterpret_cast<const float2*>(wchunk);
+                acc[0] = __ffma2_rn(sum[0], wt, acc[0]);
+                acc[1] = __ffma2_rn(sum[1], wt, acc[1]);
                 wrow ^= 64;  // a box's other chunk
                 if (c & 1) wrow += kBoxBytes;
                 xitem += 128;
                 wchunk += C::kCols;
             }
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) fence(acc[nt][i]);
+            fence(acc[0].x), fence(acc[0].y), fence(acc[1].x), fence(acc[1].y);
             __syncwarp();  // the stage is read
             if (ok) {  // else the ring stays as it is, for the end
                 if (lane == 0) {
@@ -556,20 +559,14 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
                 }
             }
         }
-        // ---- a token's three columns: v[i] of rows row (i < 2) and row + 8, tokens mt and mt + 1 (NT == 1: mt only)
-        float v[4];
-        int mt;
-        if constexpr (NT == 1) {  // columns 0 1 | 2, 3 | 4 5 of lanes t = 0, 1, 2
-            const float a = __shfl_down_sync(0xffffffffu, acc[0][0], 1), b = __shfl_down_sync(0xffffffffu, acc[0][2], 1);
-            const float c = __shfl_up_sync(0xffffffffu, acc[0][1], 1), d = __shfl_up_sync(0xffffffffu, acc[0][3], 1);
-            mt = t >> 1;
-            v[0] = t == 0 ? acc[0][0] + acc[0][1] + a : c + acc[0][0] + acc[0][1];
-            v[2] = t == 0 ? acc[0][2] + acc[0][3] + b : d + acc[0][2] + acc[0][3];
-            v[1] = v[3] = 0.0f;
-        } else {
-            mt = 2 * t;
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = acc[0][i] + acc[1][i] + acc[2][i];
+        // ---- v[i] of rows row (i < 2) and row + 8, tokens mt and mt + 1 (NT == 1: mt only)
+        float v[4] = {acc[0].x, acc[0].y, acc[1].x, acc[1].y};
+        const int mt = NT == 1 ? t >> 1 : 2 * t;
+        if constexpr (NT == 1) {  // columns 0 1 | 2, 3 | 4 5 of lanes t = 0, 1, 2: a token's three bytes
+            const float a = __shfl_down_sync(0xffffffffu, v[0], 1), b = __shfl_down_sync(0xffffffffu, v[2], 1);
+            const float c = __shfl_up_sync(0xffffffffu, v[1], 1), d = __shfl_up_sync(0xffffffffu, v[3], 1);
+            v[0] = t == 0 ? v[0] + v[1] + a : c + v[0] + v[1];
+            v[2] = t == 0 ? v[2] + v[3] + b : d + v[2] + v[3];
         }
         auto mine = [&](int i) {  // whether v[i] is an output's sum
             return NT == 1 ? (t & 1) == 0 && (i & 1) == 0 && mt < p.M : mt + (i & 1) < p.M;
