@@ -279,8 +279,11 @@ def _expect(name: str, what: str, t, shape: tuple, dtype) -> None:
         raise ValueError(f"{name}: {what} must be contiguous {list(shape)} of {dtype}, got {list(t.shape)} of {t.dtype}")
 
 
+_GROUPS = (32, 64, 128)
+
+
 def _expect_q4(name: str, q4, scales, group: int, N: int, K: int) -> None:
-    if group not in (32, 64, 128):
+    if group not in _GROUPS:
         raise ValueError(f"{name}: group must be 32, 64 or 128, got {group}")
     _expect(name, "q4", q4, (N, (K + 1) // 2), _torch.uint8)
     _expect(name, "scales", scales, (N, -(-K // group)), _torch.bfloat16)
@@ -338,24 +341,47 @@ def linear_q4(out, x, q4, scales, group: int, bias=None, stream=None) -> None:
 
 def linear_q4_add(out, x, q4, scales, group: int, bias, residual, stream=None) -> None:
     """The same plus residual[M,N] (out's type; may be out itself), added last."""
-    name = "linear_q4"
     M, K = x.shape
     N = q4.shape[0]
-    _t()
+    T, xt, ot = _torch or _t(), x.dtype, out.dtype
+    xcode, ocode = (F16 if xt is T.float16 else F32), (F16 if ot is T.float16 else F32)
+    dev = x.get_device()
+    # one pass over what has to hold; _linear_q4_refusal says what does not
+    if not (group in _GROUPS and q4.dtype is T.uint8 and q4.shape == (N, (K + 1) // 2) and q4.is_contiguous()
+            and scales.dtype is T.bfloat16 and scales.shape == (N, -(-K // group)) and scales.is_contiguous()
+            and (xt is T.float16 or xt is T.float32) and x.is_contiguous()
+            and (ot is T.float16 or ot is T.float32) and out.shape == (M, N) and out.is_contiguous()
+            and dev >= 0 and dev == out.get_device() == q4.get_device() == scales.get_device() == T.cuda.current_device()):
+        _linear_q4_refusal(out, x, q4, scales, group, bias, residual, M, N, K)
+    b = r = None
+    if bias is not None:
+        if not (bias.dtype is T.float32 and bias.shape == (N,) and bias.is_contiguous() and bias.get_device() == dev):
+            _linear_q4_refusal(out, x, q4, scales, group, bias, residual, M, N, K)
+        b = bias.data_ptr()
+    if residual is not None:
+        if not (residual.dtype is ot and residual.shape == (M, N) and residual.is_contiguous()
+                and residual.get_device() == dev):
+            _linear_q4_refusal(out, x, q4, scales, group, bias, residual, M, N, K)
+        r = residual.data_ptr()
+    status = (_lib or lib()).b200q8_linear_q4_add(out.data_ptr(), ocode, x.data_ptr(), xcode, q4.data_ptr(), scales.data_ptr(),
+                                                  group, b, r, M, N, K, _stream(stream))
+    if status:
+        _check(status)
+
+
+def _linear_q4_refusal(out, x, q4, scales, group, bias, residual, M, N, K) -> None:
+    name = "linear_q4"
     _expect_q4(name, q4, scales, group, N, K)
     _expect(name, "x", x, (M, K), x.dtype)
     _expect(name, "out", out, (M, N), out.dtype)
-    b = r = None
     if bias is not None:
         _expect(name, "bias", bias, (N,), _torch.float32)
-        b = bias.data_ptr()
     if residual is not None:
         _expect(name, "residual", residual, (M, N), out.dtype)
-        r = residual.data_ptr()
-    ocode, xcode = _float_code(name, "out", out), _float_code(name, "x", x)
+    _float_code(name, "out", out)
+    _float_code(name, "x", x)
     _same_device(name, x, out, q4, scales, bias, residual)
-    _check(lib().b200q8_linear_q4_add(out.data_ptr(), ocode, x.data_ptr(), xcode, q4.data_ptr(), scales.data_ptr(), group,
-                                      b, r, M, N, K, _stream(stream)))
+    raise AssertionError("refused without a reason")
 
 
 class _LogitRules(ctypes.Structure):
@@ -368,7 +394,10 @@ class _LogitRules(ctypes.Structure):
 def _rows_of(name: str, what: str, t, M: int, dtype):
     """(address, row stride, columns) of t: [M, n] with contiguous rows, or [n] / [1, n] shared by all rows
     (stride 0).  No columns: no address."""
-    shape, n = t.shape, t.shape[-1] if t.dim() else 0
+    shape = t.shape
+    n = shape[-1] if shape else 0
+    if len(shape) == 2 and shape[0] == M and t.dtype is dtype and t.is_contiguous():
+        return t.data_ptr() or None, (n if M > 1 else 0), n
     if t.dtype is not dtype or not (len(shape) == 2 and shape[0] in (1, M) or len(shape) == 1) or (n > 1 and t.stride(-1) != 1):
         raise ValueError(f"{name}: {what} must be [M, n] {dtype} with contiguous rows, or one such row for all, "
                          f"got {list(shape)} of {t.dtype}")
@@ -381,7 +410,8 @@ def _rows_of(name: str, what: str, t, M: int, dtype):
 def _per_row(name: str, what: str, t, M: int, dtype):
     if t is None:
         return None
-    _expect(name, what, t, (M,), dtype)
+    if t.dtype is not dtype or t.shape != (M,) or not t.is_contiguous():
+        _expect(name, what, t, (M,), dtype)
     return t.data_ptr()
 
 
@@ -397,8 +427,9 @@ def process_logits(out, logits, argmax=None, history=None, history_len=None, pro
     name = "process_logits"
     M, V = logits.shape
     i32, f32 = _t().int32, _torch.float32
-    if V > 1 and (logits.stride(1) != 1 or (out is not None and out.stride(-1) != 1)) or (
-            out is not None and out.shape != (M, V)):
+    xs = logits.stride()
+    os_ = xs if out is logits or out is None else out.stride()
+    if V > 1 and (xs[1] != 1 or os_[-1] != 1) or (out is not None and out.shape != (M, V)):
         raise ValueError(f"{name}: logits and out must be [{M}, {V}] with contiguous rows")
     am = _per_row(name, "argmax", argmax, M, i32)
     rules = None
@@ -428,9 +459,11 @@ def process_logits(out, logits, argmax=None, history=None, history_len=None, pro
     if out is None:
         to, ocode, ostride = None, xcode, V
     else:
-        to, ocode, ostride = out.data_ptr(), _float_code(name, "out", out), out.stride(0) if M > 1 else V
-    _check(lib().b200q8_process_logits(to, ocode, ostride, logits.data_ptr(), xcode, logits.stride(0) if M > 1 else V, M, V,
-                                       None if rules is None else ctypes.addressof(rules), am, _stream(stream)))
+        to, ocode, ostride = out.data_ptr(), _float_code(name, "out", out), os_[0] if M > 1 else V
+    status = (_lib or lib()).b200q8_process_logits(to, ocode, ostride, logits.data_ptr(), xcode, xs[0] if M > 1 else V, M, V,
+                                                   None if rules is None else ctypes.addressof(rules), am, _stream(stream))
+    if status:
+        _check(status)
 
 
 ST_F32, ST_F16, ST_BF16, ST_I8, ST_OTHER = 0, 1, 2, 3, 4
