@@ -148,6 +148,18 @@ __device__ __forceinline__ void lds(uint32_t a, uint32_t (&w)[W])
     else
         asm("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
 }
+// N words from global memory in one load.
+__device__ __forceinline__ void load_words(const uint16_t* p, uint32_t (&w)[1]) { w[0] = __ldg(reinterpret_cast<const uint32_t*>(p)); }
+__device__ __forceinline__ void load_words(const uint16_t* p, uint32_t (&w)[2])
+{
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    w[0] = v.x, w[1] = v.y;
+}
+__device__ __forceinline__ void load_words(const uint16_t* p, uint32_t (&w)[4])
+{
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+}
 __device__ __forceinline__ void fence(uint32_t& v) { asm volatile("" : "+r"(v)::"memory"); }
 __device__ __forceinline__ void fence(float& v) { asm volatile("" : "+f"(v)::"memory"); }
 
@@ -341,6 +353,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     constexpr int kItemBytes = C::kItemBytes;
     constexpr int W = G / 32;   // words a lane holds of a group; 32-blocks of a group
     constexpr int GC = 128 / G;  // groups of a chunk
+    constexpr int kBoxGroups = kBoxK / G;
     namespace cg = cooperative_groups;
     const cg::cluster_group cluster = cg::this_cluster();
     const int csize = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -407,36 +420,55 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
             tc::tma_load_2d_hint(ring + stage * kItemBytes + b * kBoxBytes, &tmW, (ich * IB + b) * 128, itile * 16,
                                  bar0 + 8 * stage, policy);
     };
-    // Scales of the chunk about to be multiplied, two to a word, loaded while the one before is.
-    constexpr int kSW = (GC + 1) / 2;
-    uint32_t sc0[kSW], sc1[kSW];
-    const uint16_t* sp = nullptr;  // of the fragment's first row; the other row's lie `srow` behind
-    size_t srow = 0;
-    int sg = 0;  // group index that sp points at
-    const bool swide = GC == 4 && ng % 4 == 0 && ((uintptr_t)p.a.scales & 7) == 0;  // four scales in one load
-    auto load_scales = [&]() {
-        if (GC == 4 && swide) {
-            const uint2 a = sg < ng ? __ldg(reinterpret_cast<const uint2*>(sp)) : make_uint2(0, 0);
-            const uint2 b = sg < ng ? __ldg(reinterpret_cast<const uint2*>(sp + srow)) : make_uint2(0, 0);
-            sc0[0] = a.x, sc1[0] = b.x;
-            if constexpr (kSW == 2) sc0[1] = a.y, sc1[1] = b.y;
+    // Scales, two to a word, of the box about to be multiplied and of the next; those of the one after are
+    // loaded meanwhile (a box takes less than a load from L2).
+    constexpr int kSW = kBoxGroups / 2;
+    struct Scales {
+        uint32_t a[kSW], b[kSW];  // the fragment's two rows
+    };
+    int stile = busy ? tile0 : p.tiles, sch = ch0 + kw, sbox = 0;  // the box whose scales are loaded next
+    const uint16_t* sp = nullptr;
+    size_t srow = 0;  // from the first row's scales to the other's
+    const bool swide = ng % kBoxGroups == 0 && ((uintptr_t)p.a.scales & (2 * kBoxGroups - 1)) == 0;  // one load a row
+    auto load_scales = [&](Scales& s) {
+        if (stile >= p.tiles) return;
+        if (sbox == 0 && sch == ch0 + kw) {
+            const int n0 = min(stile * 16 + row, N - 1), n1 = min(stile * 16 + row + 8, N - 1);
+            sp = p.a.scales + (size_t)n0 * ng + sch * IB * kBoxGroups;
+            srow = (size_t)(n1 - n0) * ng;
+        }
+        const int g0 = (sch * IB + sbox) * kBoxGroups;
+        if (swide) {
+            if (g0 < ng) {
+                load_words(sp, s.a);
+                load_words(sp + srow, s.b);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kSW; i++) s.a[i] = s.b[i] = 0;
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < GC; i++) {
-                const bool in = sg + i < ng;  // a row's last item may be short
+            for (int i = 0; i < kBoxGroups; i++) {
+                const bool in = g0 + i < ng;  // a row's last box may be short
                 const uint32_t a = in ? (uint32_t)__ldg(sp + i) : 0u, b = in ? (uint32_t)__ldg(sp + srow + i) : 0u;
-                sc0[i / 2] = i & 1 ? sc0[i / 2] | a << 16 : a;
-                sc1[i / 2] = i & 1 ? sc1[i / 2] | b << 16 : b;
+                s.a[i / 2] = i & 1 ? s.a[i / 2] | a << 16 : a;
+                s.b[i / 2] = i & 1 ? s.b[i / 2] | b << 16 : b;
+            }
+        }
+        if (++sbox < IB) {
+            sp += kBoxGroups;
+        } else {
+            sbox = 0;
+            sch += wk;
+            sp += ((wk - 1) * IB + 1) * kBoxGroups;
+            if (sch >= ch1) {
+                sch = ch0 + kw;
+                stile += tstep;
             }
         }
     };
-    auto first_scales = [&](int tile) {
-        const int n0 = min(tile * 16 + row, N - 1), n1 = min(tile * 16 + row + 8, N - 1);
-        sg = (ch0 + kw) * C::kChunks * GC;
-        sp = p.a.scales + (size_t)n0 * ng + sg;
-        srow = (size_t)(n1 - n0) * ng;
-        load_scales();
-    };
+    Scales sc{}, sc_next{};
+
     // The tokens' loads go first and one item a warp behind them, the others once the tokens are done: behind
     // more the loads would wait for megabytes to pass (37888 x 3584, one token: 14.9 us; all items first 16.5).
     const bool some = stage_tokens<NT>(xs, weight, direct, p, W, ch0 * C::kChunks * 4, xchunks * 4, [&]() {
@@ -444,7 +476,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
             load_item(inflight++);
             advance();
         }
-        if (busy && tile0 < p.tiles) first_scales(tile0);
+        load_scales(sc);
+        load_scales(sc_next);
     });
     if (lane == 0)
         for (; inflight < p.stages && itile < p.tiles; inflight++, advance()) load_item(inflight);
@@ -482,65 +515,60 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
             const float* wchunk = weight + (ch - ch0) * C::kChunks * C::kCols + 2 * t;
             // Chunks behind K need no care: their codes and tokens are zeros, and so are their scales.
 #pragma unroll 1
-            for (int c = 0; c < C::kChunks; c++) {
-                float s0[GC], s1[GC];
+            for (int box = 0; box < IB; box++) {
+                Scales sc_after = sc_next;
+                load_scales(sc_after);
 #pragma unroll
-                for (int i = 0; i < GC; i++) {
-                    s0[i] = __uint_as_float(i & 1 ? sc0[i / 2] & 0xFFFF0000u : sc0[i / 2] << 16);
-                    s1[i] = __uint_as_float(i & 1 ? sc1[i / 2] & 0xFFFF0000u : sc1[i / 2] << 16);
-                }
-                if (c + 1 < C::kChunks || ch + wk < ch1) {
-                    const int step = c + 1 < C::kChunks ? GC : ((wk - 1) * C::kChunks + 1) * GC;
-                    sp += step, sg += step;
-                    load_scales();
-                } else if (tile + tstep < p.tiles) {
-                    first_scales(tile + tstep);
-                }
-                uint32_t x[NT][2][4];
+                for (int c = 0; c < 2; c++) {
+                    uint32_t x[NT][2][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    lds<4>(xoff[nt] + xitem, x[nt][0]);
-                    lds<4>(xoff[nt] + xitem + 64, x[nt][1]);
-                }
-                float2 sum[2];
+                    for (int nt = 0; nt < NT; nt++) {
+                        lds<4>(xoff[nt] + xitem + c * 128, x[nt][0]);
+                        lds<4>(xoff[nt] + xitem + c * 128 + 64, x[nt][1]);
+                    }
+                    float2 sum[2];
 #pragma unroll
-                for (int gi = 0; gi < GC; gi++) {
-                    uint32_t w0[W], w1[W];
-                    lds<W>(wrow ^ (gi * W * 16), w0);
-                    lds<W>((wrow ^ (gi * W * 16)) + 1024, w1);
-                    int d[NT][4];
+                    for (int gi = 0; gi < GC; gi++) {
+                        uint32_t w0[W], w1[W];
+                        lds<W>(wrow ^ (c * 64 + gi * W * 16), w0);
+                        lds<W>((wrow ^ (c * 64 + gi * W * 16)) + 1024, w1);
+                        int d[NT][4];
 #pragma unroll
-                    for (int b = 0; b < W; b++) {
-                        const int blk = gi * W + b;
-                        uint32_t a0, a1, a2, a3;
-                        unpack8(w0[b], a0, a2);
-                        unpack8(w1[b], a1, a3);
+                        for (int b = 0; b < W; b++) {
+                            const int blk = gi * W + b;
+                            uint32_t a0, a1, a2, a3;
+                            unpack8(w0[b], a0, a2);
+                            unpack8(w1[b], a1, a3);
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            const uint32_t b0 = x[nt][blk >> 1][2 * (blk & 1)], b1 = x[nt][blk >> 1][2 * (blk & 1) + 1];
-                            if (b == 0)
-                                mma16832<true>(d[nt], kMagicBits, a0, a1, a2, a3, b0, b1);
-                            else
-                                mma16832<false>(d[nt], 0, a0, a1, a2, a3, b0, b1);
+                            for (int nt = 0; nt < NT; nt++) {
+                                const uint32_t b0 = x[nt][blk >> 1][2 * (blk & 1)], b1 = x[nt][blk >> 1][2 * (blk & 1) + 1];
+                                if (b == 0)
+                                    mma16832<true>(d[nt], kMagicBits, a0, a1, a2, a3, b0, b1);
+                                else
+                                    mma16832<false>(d[nt], 0, a0, a1, a2, a3, b0, b1);
+                            }
+                        }
+                        const int si = c * GC + gi;
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const uint32_t word = i == 0 ? sc.a[si / 2] : sc.b[si / 2];
+                            const float r = __uint_as_float(si & 1 ? word & 0xFFFF0000u : word << 16);
+                            float2 f = tile_value(d[0], i);
+                            if constexpr (NT == 3)  // X0 + 256 X1 + 65536 X2
+                                f = __ffma2_rn(__ffma2_rn(tile_value(d[2], i), make_float2(256.0f, 256.0f), tile_value(d[1], i)),
+                                               make_float2(256.0f, 256.0f), f);
+                            sum[i] = gi == 0 ? __fmul2_rn(f, make_float2(r, r)) : __ffma2_rn(f, make_float2(r, r), sum[i]);
                         }
                     }
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const float r = i == 0 ? s0[gi] : s1[gi];
-                        float2 f = tile_value(d[0], i);
-                        if constexpr (NT == 3)  // X0 + 256 X1 + 65536 X2
-                            f = __ffma2_rn(__ffma2_rn(tile_value(d[2], i), make_float2(256.0f, 256.0f), tile_value(d[1], i)),
-                                           make_float2(256.0f, 256.0f), f);
-                        sum[i] = gi == 0 ? __fmul2_rn(f, make_float2(r, r)) : __ffma2_rn(f, make_float2(r, r), sum[i]);
-                    }
+                    const float2 wt = *reinterpret_cast<const float2*>(wchunk + c * C::kCols);
+                    acc[0] = __ffma2_rn(sum[0], wt, acc[0]);
+                    acc[1] = __ffma2_rn(sum[1], wt, acc[1]);
                 }
-                const float2 wt = *reinterpret_cast<const float2*>(wchunk);
-                acc[0] = __ffma2_rn(sum[0], wt, acc[0]);
-                acc[1] = __ffma2_rn(sum[1], wt, acc[1]);
-                wrow ^= 64;  // a box's other chunk
-                if (c & 1) wrow += kBoxBytes;
-                xitem += 128;
-                wchunk += C::kCols;
+                sc = sc_next;
+                sc_next = sc_after;
+                wrow += kBoxBytes;
+                xitem += 256;
+                wchunk += 2 * C::kCols;
             }
             fence(acc[0].x), fence(acc[0].y), fence(acc[1].x), fence(acc[1].y);
             __syncwarp();  // the stage is read
