@@ -114,12 +114,15 @@ struct ScratchNeed {
     bool amax = false;
 };
 
-// Grows one device buffer of `s` to at least `need` elements (never shrinks).
+// Grows one device buffer of `s` to at least `need` elements (never shrinks).  The buffer it replaces is kept
+// until exit: a graph captured earlier may still hold it.  Sizes at least double, so those kept add up to
+// less than the one in use.
 template <typename T>
 int grow(T** buf, size_t* have, size_t need, size_t dflt, cudaStream_t stream, bool zero, const char* what)
 {
     if (*have >= need) return B200Q8_OK;
-    const size_t n = need > dflt ? need : dflt;
+    size_t n = need > dflt ? need : dflt;
+    if (n < 2 * *have) n = 2 * *have;
     T* nb = nullptr;
     cudaError_t e = cudaMalloc(&nb, n * sizeof(T));
     if (e != cudaSuccess) {
@@ -130,22 +133,27 @@ int grow(T** buf, size_t* have, size_t need, size_t dflt, cudaStream_t stream, b
         cudaFree(nb);
         return cuda_fail(e, "scratch memset");
     }
-    if (*buf) {  // the old buffer may still be in use by queued work on this stream
-        cudaStreamSynchronize(stream);
-        cudaFree(*buf);
-    }
     *buf = nb;
     *have = n;
     return B200Q8_OK;
 }
 
-int get_scratch(const ScratchNeed& need, int num_sms, cudaStream_t stream, TcScratch* out)
+// capture_ok false: a call that would have to allocate during a capture is refused (the allocation would
+// end the capture) instead of attempted.
+int get_scratch(const ScratchNeed& need, int num_sms, cudaStream_t stream, TcScratch* out, bool capture_ok = true)
 {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
     std::lock_guard<std::mutex> lk(g_scratch_mu);
     TcScratch& s = g_scratch[ScratchKey{dev, stream}];
+    if (!capture_ok && (s.ws_floats < need.ws || s.counters < need.counters || s.act_bytes < need.act)) {
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess) cudaGetLastError();
+        if (capture != cudaStreamCaptureStatusNone)
+            return fail(B200Q8_ERR_ALLOC, "this call would have to allocate scratch, which a stream capture does not "
+                        "allow: make a call of the same shape on this stream before the capture");
+    }
     // Default capacities: 128-column partials on every SM, 64K tiles.
     int st;
     if ((st = grow(&s.ws, &s.ws_floats, need.ws, (size_t)2 * num_sms * 128 * 128, stream, false, "partials")) ||
@@ -337,7 +345,7 @@ int stream_scratch(size_t ws_floats, size_t counters, size_t act_bytes, int num_
     need.ws = ws_floats;
     need.counters = counters;
     need.act = act_bytes;
-    return get_scratch(need, num_sms, stream, out);
+    return get_scratch(need, num_sms, stream, out, false);
 }
 
 int current_device(int* num_sms, size_t* max_smem)

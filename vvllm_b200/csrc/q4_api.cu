@@ -2,7 +2,6 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
-#include <cstdlib>
 
 #include "b200q8.h"
 #include "kernels.h"
@@ -96,9 +95,14 @@ int linear_q4(const char* what, void* out, int out_dtype, const void* inp, int i
     a.group = group;
     a.in_dtype = in_dtype;
     a.out_dtype = out_dtype;
+    // Up to 8 tokens the streaming kernel reads the weights once; above, once for every 8, where the GEMM
+    // (fp16 tokens) reads them once at a rate bound by its dequantization.  Measured on B200, streaming vs GEMM:
+    // 37888 x 3584 at 8 tokens 23 vs 37 us, at 9 37 vs 38, at 16 46 vs 38; 3584 x 18944 at 8 33 vs 28, at 16 65 vs 28.
+    // For 9 to 16 tokens and few weights with a long K, of which the GEMM makes few tiles, two passes still
+    // win: 3584 x 3584 at 16 19 vs 19, 896 x 4864 23 vs 24, 512 x 18944 29 vs 32; not 4864 x 896, 14 vs 10.
+    const bool gemm = M > 16 || (M > 8 && (N * K > ((size_t)1 << 24) || K < 2048));
     cudaError_t e;
-    static const int kGemmMin = getenv("Q4_GEMM") ? atoi(getenv("Q4_GEMM")) : 9;
-    if (M >= (size_t)kGemmMin && q4_gemm_tc_supports(a)) {
+    if (gemm && q4_gemm_tc_supports(a)) {
         size_t ws = 0, counters = 0, act = 0;
         q4_gemm_tc_scratch_need(a, sms, &ws, &counters, &act);
         TcScratch scratch;

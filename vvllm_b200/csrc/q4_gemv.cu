@@ -215,87 +215,104 @@ __device__ __forceinline__ int column_of(int m, int d, int M)  // where it is st
 //           w of lane t starts at element (t * W + w) * 8.  Zero behind K.
 //   weight  [chunk][8]: what a column's integer (NT == 1; else a token's X) counts, with the 1/16 of the codes' bytes
 //   direct  [token][chunk]: 1 if the chunk is summed directly; returns whether this thread saw any
-// Half a warp per chunk of 128 elements, eight elements a lane; a few chunks' loads at a time.  `then` is
-// called once the first loads are under way.
-template <int NT, class Then>
+// Half a warp per chunk of 128 elements, eight elements a lane; a few chunks' loads at a time.  `asked` is
+// called once the first loads are under way, `arrived` once they are there.
+template <int NT, bool kF16, class Asked, class Arrived>
 __device__ __forceinline__ bool stage_tokens(unsigned char* xs, float* weight, unsigned char* direct,
-                                             const StreamParams& p, int W, int block0, int blocks, Then then)
+                                             const StreamParams& p, int W, int block0, int blocks, Asked asked, Arrived arrived)
 {
-    constexpr int U = 4;  // chunks whose loads are in flight
+    constexpr int U = 5;  // chunks whose loads are in flight
+    constexpr int kRaw = kF16 ? 4 : 8;
     const int K = (int)p.a.K, chunks = blocks / 4;
     const size_t cs = column_stride(blocks);
     const int u = threadIdx.x & 15;  // word of the chunk
-    bool any = false;
-    const int total = chunks * p.M, half = threadIdx.x >> 4, halves = blockDim.x >> 4;
-    const bool f16 = p.a.in_dtype == kF16;
-    for (int i0 = half; i0 - half < total; i0 += U * halves) {  // whole warps: the shuffles below
-        uint4 raw[U][2];
+    const int half = threadIdx.x >> 4, halves = blockDim.x >> 4;
+    const int o = u & (4 * W - 1), ub = u / (4 * W) * W + (o & (W - 1));  // its block in the chunk
+    unsigned char* const dst0 = xs + (ub >> 1) * 64 + (o / W) * 16 + (ub & 1) * 8;
+    bool any = false, first = true;
+    // Rounds: every half warp a chunk of one token, chunks c0 + half.
+    for (int m = 0, c0 = 0; m < p.M;) {
+        uint32_t raw[U][kRaw];
+        int lm = m, lc = c0;
 #pragma unroll
         for (int q = 0; q < U; q++) {
-            const int i = i0 + q * halves, m = i / chunks, k = block0 * 32 + (i - m * chunks) * 128 + u * 8;
-            raw[q][0] = raw[q][1] = make_uint4(0, 0, 0, 0);
-            if (i < total && k < K) {
-                if (f16) {
-                    raw[q][0] = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.a.x) + (size_t)m * K + k);
-                } else {
-                    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(p.a.x) + (size_t)m * K + k);
-                    raw[q][0] = src[0];
-                    raw[q][1] = src[1];
+            const int k = block0 * 32 + (lc + half) * 128 + u * 8;
+#pragma unroll
+            for (int j = 0; j < kRaw; j++) raw[q][j] = 0;
+            if (lm < p.M && lc + half < chunks && k < K) {
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const char*>(p.a.x) +
+                                                                  ((size_t)lm * K + k) * (kF16 ? 2 : 4));
+#pragma unroll
+                for (int j = 0; j < kRaw / 4; j++) {
+                    const uint4 r = src[j];
+                    raw[q][4 * j] = r.x, raw[q][4 * j + 1] = r.y, raw[q][4 * j + 2] = r.z, raw[q][4 * j + 3] = r.w;
                 }
             }
+            lc += halves;
+            if (lc >= chunks) lc = 0, lm++;
         }
-        if (i0 == half) then();
+        if (first) asked();
 #pragma unroll
         for (int q = 0; q < U; q++) {
-            const int i = i0 + q * halves, m = i / chunks, c = i - m * chunks;
-            if (i - half >= total) break;  // uniform in the CTA
+            if (m >= p.M) break;  // uniform in the CTA
+            // The largest |x| as bits: above every number for an infinity or NaN.
             float v[8];
-            if (f16) {
-                const uint32_t h[4] = {raw[q][0].x, raw[q][0].y, raw[q][0].z, raw[q][0].w};
+            uint32_t top;
+            if constexpr (kF16) {
+                uint32_t h = 0;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+                    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(h) : "r"(raw[q][j] & 0x7FFF7FFFu));
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&raw[q][j]));
                     v[2 * j] = f.x, v[2 * j + 1] = f.y;
                 }
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                top = max(__float_as_uint(f.x), __float_as_uint(f.y));
             } else {
-                const uint4 lo = raw[q][0], hi = raw[q][1];
-                v[0] = __uint_as_float(lo.x), v[1] = __uint_as_float(lo.y), v[2] = __uint_as_float(lo.z);
-                v[3] = __uint_as_float(lo.w), v[4] = __uint_as_float(hi.x), v[5] = __uint_as_float(hi.y);
-                v[6] = __uint_as_float(hi.z), v[7] = __uint_as_float(hi.w);
+                top = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    v[j] = __uint_as_float(raw[q][j]);
+                    top = max(top, raw[q][j] & 0x7FFFFFFFu);
+                }
             }
-            uint32_t top = 0;  // largest |x| as bits: above every number for an infinity or NaN
 #pragma unroll
-            for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+            if (first) arrived();
+            first = false;
             const bool bad = top >= 0x7F800000u;
             const int e = max((int)(top >> 23) - 126, -100);  // |x| < 2^e
-            const float up = bad ? 0.0f : __uint_as_float((uint32_t)(22 - e + 127) << 23);
+            const float up = __uint_as_float((uint32_t)(22 - e + 127) << 23);
             // X in the low bits of x * up + 1.5 * 2^23; with 128 added to each byte, the bytes are the signed
             // digits with their top bit flipped.
             uint32_t y[8];
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                y[j] = __float_as_uint(bad ? kMagic : fmaf(v[j], up, kMagic)) + (0x00808080u - (uint32_t)kMagicBits);
-            uint32_t d[3][2];  // digit, even / odd elements
+                y[j] = __float_as_uint(fmaf(v[j], up, kMagic)) + (0x00808080u - (uint32_t)kMagicBits);
+            if (bad)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint32_t lo = __byte_perm(y[h], y[2 + h], 0x5140), hi = __byte_perm(y[4 + h], y[6 + h], 0x5140);
-                d[0][h] = __byte_perm(lo, hi, 0x5410) ^ 0x80808080u;
-                d[1][h] = __byte_perm(lo, hi, 0x7632) ^ 0x80808080u;
-                d[2][h] = __byte_perm(__byte_perm(y[h], y[2 + h], 0x0062), __byte_perm(y[4 + h], y[6 + h], 0x0062), 0x5410) ^ 0x80808080u;
-            }
-            const int o = u & (4 * W - 1), b = c * 4 + u / (4 * W) * W + (o & (W - 1)), t = o / W;
-            unsigned char* dst = xs + (b >> 1) * 64 + t * 16 + (b & 1) * 8;
-            if (i < total) {
+                for (int j = 0; j < 8; j++) y[j] = 0x00808080u;
+            const int c = c0 + half;
+            if (c < chunks) {
+                unsigned char* dst = dst0 + c * 128;
 #pragma unroll
-                for (int n = 0; n < 3; n++)
-                    *reinterpret_cast<uint2*>(dst + column_of<NT>(m, n, p.M) * cs) = make_uint2(d[n][0], d[n][1]);
+                for (int n = 0; n < 3; n++) {
+                    uint32_t d[2];  // the digit of the even and the odd elements
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t lo = __byte_perm(y[h], y[2 + h], n == 2 ? 0x0062 : 0x5140);
+                        const uint32_t hi = __byte_perm(y[4 + h], y[6 + h], n == 2 ? 0x0062 : 0x5140);
+                        d[h] = __byte_perm(lo, hi, n == 1 ? 0x7632 : 0x5410) ^ 0x80808080u;
+                    }
+                    *reinterpret_cast<uint2*>(dst + column_of<NT>(m, n, p.M) * cs) = make_uint2(d[0], d[1]);
+                }
                 if (u < (NT == 1 ? 3 : 1))
                     weight[c * 8 + (NT == 1 ? 3 * m + u : m)] = __uint_as_float((uint32_t)(e - 22 - 4 + 8 * u + 127) << 23);
                 if (u == 3) direct[m * chunks + c] = bad;
                 any |= bad;
             }
+            c0 += halves;
+            if (c0 >= chunks) c0 = 0, m++;
         }
     }
     return any;
@@ -469,18 +486,24 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     };
     Scales sc{}, sc_next{};
 
-    // The tokens' loads go first and one item a warp behind them, the others once the tokens are done: behind
-    // more the loads would wait for megabytes to pass (37888 x 3584, one token: 14.9 us; all items first 16.5).
-    const bool some = stage_tokens<NT>(xs, weight, direct, p, W, ch0 * C::kChunks * 4, xchunks * 4, [&]() {
+    // The tokens' loads go first, then one item a warp: behind more they would wait for megabytes to pass (all of
+    // the ring first: 16.5 us for 37888 x 3584 and one token, instead of 14).  Once they are there the ring is
+    // filled, before they are converted.  (Requesting two more items into L2 as well: 14.8 us.)
+    auto asked = [&]() {
         if (lane == 0 && itile < p.tiles) {
             load_item(inflight++);
             advance();
         }
         load_scales(sc);
         load_scales(sc_next);
-    });
-    if (lane == 0)
-        for (; inflight < p.stages && itile < p.tiles; inflight++, advance()) load_item(inflight);
+    };
+    auto arrived = [&]() {
+        if (lane == 0)
+            for (; inflight < p.stages && itile < p.tiles; inflight++, advance()) load_item(inflight);
+    };
+    const bool some = p.a.in_dtype == kF16
+                          ? stage_tokens<NT, true>(xs, weight, direct, p, W, ch0 * C::kChunks * 4, xchunks * 4, asked, arrived)
+                          : stage_tokens<NT, false>(xs, weight, direct, p, W, ch0 * C::kChunks * 4, xchunks * 4, asked, arrived);
     const bool any_direct = __syncthreads_or(some);
     if (csize > 1) cluster.sync();  // every rank runs before rank 0's memory is stored to
 
