@@ -38,6 +38,7 @@ namespace b200q8 {
 namespace {
 
 constexpr int kThreads = 512;
+constexpr size_t kStaticSmem = 4096;  // left to the kernel's static shared memory
 
 // Unsigned key of a float that is no NaN: larger value, larger key; -0 and +0 alike.
 __device__ __forceinline__ uint32_t order_key(float v)
@@ -485,15 +486,18 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitArgs a, 
     }
 }
 
-template <typename IT, typename OT, bool kWide, int C>
-cudaError_t launch_sized(const LogitArgs& a, size_t max_smem, cudaStream_t stream)
+struct Plan {
+    int room;     // blocks of a CTA that its slots hold at a time
+    size_t smem;  // dynamic shared memory
+};
+
+template <bool kWide, int C>
+Plan plan(const LogitArgs& a, size_t max_smem)
 {
-    auto kern = logits_kernel<IT, OT, kWide, C>;
     constexpr size_t kBytes = Slots<kWide>::kBytes;
     using Listed = typename Slots<kWide>::Listed;
     const size_t lists = (a.history ? 1 : 0) + (a.bias_ids ? 1 : 0);
-    const size_t budget = max_smem - 4096;  // beside the static part
-    long long room = (((long long)a.V + kBlock - 1) / kBlock + C - 1) / C;  // blocks of a CTA
+    long long room = (((long long)a.V + kBlock - 1) / kBlock + C - 1) / C;
     size_t smem = 0;
     if (lists) {
         if (!kWide) room = std::min<long long>(room, 63);  // slot numbers of 16 bits
@@ -501,23 +505,31 @@ cudaError_t launch_sized(const LogitArgs& a, size_t max_smem, cudaStream_t strea
         for (;; room--) {  // one block always fits
             const size_t tokens = (size_t)room * kBlock;
             smem = (tokens / 32 + 4) * 4 + lists * (tokens + 8) * kBytes + std::min(most, tokens + 4) * sizeof(Listed);
-            if (smem <= budget) break;
+            if (smem <= max_smem - kStaticSmem) break;
         }
     }
+    return {(int)room, smem};
+}
+
+template <typename IT, typename OT, bool kWide, int C>
+cudaError_t launch_sized(const LogitArgs& a, size_t max_smem, cudaStream_t stream)
+{
+    auto kern = logits_kernel<IT, OT, kWide, C>;
+    const Plan s = plan<kWide, C>(a, max_smem);
     static thread_local bool configured[64] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!configured[dev]) {
-        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)budget);
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(max_smem - kStaticSmem));
         if (e != cudaSuccess) return e;
         configured[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.M * C));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = s.smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -527,7 +539,7 @@ cudaError_t launch_sized(const LogitArgs& a, size_t max_smem, cudaStream_t strea
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, kern, a, (int)room);
+    e = cudaLaunchKernelEx(&cfg, kern, a, s.room);
     if (e == cudaSuccess) note_launch();
     return e;
 }
@@ -536,7 +548,10 @@ template <typename IT, typename OT>
 cudaError_t launch_typed(const LogitArgs& a, int num_sms, size_t max_smem, cudaStream_t stream)
 {
     const bool wide = (a.history && a.history_count > 32767) || (a.bias_ids && a.bias_count > 65534);
-    const bool eight = a.M * 8 <= (size_t)num_sms * 2;  // as many CTAs as find room at a time
+    // Eight CTAs a row while they all find room at a time, and where four would be too large for two to an SM
+    // (64 rows of 152064 with histories of 4096 and 300 biases: 36 us, with four 42; without biases 32 and 27).
+    const bool eight = a.M * 8 <= (size_t)num_sms * 2 ||
+                       (wide ? plan<true, 4>(a, max_smem) : plan<false, 4>(a, max_smem)).smem > 112 * 1024;
     if (wide)
         return eight ? launch_sized<IT, OT, true, 8>(a, max_smem, stream) : launch_sized<IT, OT, true, 4>(a, max_smem, stream);
     return eight ? launch_sized<IT, OT, false, 8>(a, max_smem, stream) : launch_sized<IT, OT, false, 4>(a, max_smem, stream);

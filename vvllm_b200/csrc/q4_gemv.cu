@@ -353,11 +353,13 @@ struct StreamCfg {
     static constexpr int kChunks = IB * kBoxK / 128;  // 128-chunks of an item
     static constexpr int kCols = 8;                   // columns kept in `weight`: NT == 1 the tile's, else the tokens
     static constexpr int kSums = NT == 1 ? 2 * 16 : 8 * 16;  // a tile's outputs: [token][row]
-    static size_t smem(int warps, int stages, int M, int per, int cluster)
+    // Two buffers of sums, read while the next tile's are written, where warps or CTAs share a tile.
+    static constexpr int red_bufs(int wk, int cluster) { return wk == 1 && cluster == 1 ? 1 : 2; }
+    static size_t smem(int warps, int stages, int M, int per, int cluster, int wk)
     {
         const int chunks = per * kChunks;
         return 1024 + (size_t)warps * stages * kItemBytes + warps * kMaxStages * 8 + 3 * M * column_stride(chunks * 4) +
-               (size_t)chunks * kCols * 4 + (size_t)2 * warps * kSums * 4 +
+               (size_t)chunks * kCols * 4 + (size_t)red_bufs(wk, cluster) * warps * kSums * 4 +
                (cluster > 1 ? (size_t)2 * cluster * kSums * 4 : 0) + (size_t)M * chunks;
     }
 };
@@ -384,8 +386,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     const int xchunks = p.per * C::kChunks;
     const size_t cs = column_stride(xchunks * 4);
     float* weight = reinterpret_cast<float*>(xs + 3 * p.M * cs);
-    float* red = weight + xchunks * C::kCols;         // [2][warp][tile's outputs]
-    float* cbuf = red + 2 * warps * C::kSums;         // [2][rank][tile's outputs] of a cluster's CTAs (in rank 0)
+    float* red = weight + xchunks * C::kCols;         // [buffer][warp][tile's outputs]
+    float* cbuf = red + C::red_bufs(p.wk, csize) * warps * C::kSums;  // [2][rank][tile's outputs] of a cluster's CTAs (in rank 0)
     unsigned char* direct = reinterpret_cast<unsigned char*>(cbuf + (csize > 1 ? 2 * csize * C::kSums : 0));
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -684,7 +686,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
                 __syncwarp();
             }
         }
-        parity ^= 1;  // one buffer is read while the next tile's sums go to the other
+        if (wk == 1 && csize == 1)
+            __syncwarp();  // the one buffer is read
+        else
+            parity ^= 1;
     }
     if (!ok && lane == 0)  // copies still in flight land before the CTA ends
         for (int i = 0; i < inflight; i++) {
@@ -733,7 +738,7 @@ cudaError_t launch_stream(const StreamParams& p, const StreamPlan& s, int num_sm
     const int groups = s.warps / p.wk;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3((unsigned)s.warps * 32);
-    cfg.dynamicSmemBytes = C::smem(s.warps, p.stages, p.M, p.per, s.cluster);
+    cfg.dynamicSmemBytes = C::smem(s.warps, p.stages, p.M, p.per, s.cluster, p.wk);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -782,57 +787,69 @@ cudaError_t launch_stream_nt(const StreamParams& p, const StreamPlan& s, int num
     if (s.nt == 1)
         return s.ib == 1 ? launch_stream<1, G, 1>(p, s, num_sms, max_smem, stream)
                          : launch_stream<1, G, 2>(p, s, num_sms, max_smem, stream);
-    return launch_stream<3, G, 1>(p, s, num_sms, max_smem, stream);
+    return s.ib == 1 ? launch_stream<3, G, 1>(p, s, num_sms, max_smem, stream)
+                     : launch_stream<3, G, 2>(p, s, num_sms, max_smem, stream);
 }
 
-size_t stream_smem(int nt, int ib, int warps, int stages, int M, int per, int cluster)
+size_t stream_smem(int nt, int ib, int warps, int stages, int M, int per, int cluster, int wk)
 {
     if (nt == 1)
-        return ib == 1 ? StreamCfg<1, 1>::smem(warps, stages, M, per, cluster) : StreamCfg<1, 2>::smem(warps, stages, M, per, cluster);
-    return StreamCfg<3, 1>::smem(warps, stages, M, per, cluster);
+        return ib == 1 ? StreamCfg<1, 1>::smem(warps, stages, M, per, cluster, wk)
+                       : StreamCfg<1, 2>::smem(warps, stages, M, per, cluster, wk);
+    return ib == 1 ? StreamCfg<3, 1>::smem(warps, stages, M, per, cluster, wk)
+                   : StreamCfg<3, 2>::smem(warps, stages, M, per, cluster, wk);
 }
 
 constexpr int kMaxCluster = 8;
 
+// Items of two boxes where a row has several (a wait, a copy and their bookkeeping cost about as much as a
+// box's products: 37888 x 3584, one token, 15.8 us with one box, 14.9 with two), two items in flight a warp
+// (three: 16.4 us, the copies' queue then holds up the warps); two CTAs of 8 warps an SM where the tokens
+// leave room, else one of 16, else one of 8; a cluster only where one CTA cannot hold the tokens (it measured slower
+// wherever both were possible).
 StreamPlan plan_stream(const Q4Args& a, size_t M, int num_sms, size_t max_smem)
 {
     StreamPlan s;
     const int tiles = (int)((a.N + 15) / 16);
     for (int m = (int)std::min<size_t>(M, kMaxTokens); m >= 1 && !s.tokens; m--) {
         const int nt = m <= 2 ? 1 : 3;
-        const int ib = a.K >= 2048 && nt == 1 ? 2 : 1;
-        const int nch = (int)((a.K + ib * kBoxK - 1) / (ib * kBoxK));
-        for (int c = 1; c <= kMaxCluster && !s.tokens; c *= 2) {
-            const int per = (nch + c - 1) / c;
-            if ((nch + per - 1) / per != c) continue;  // a rank would have nothing
-            auto fit = [&](int warps, size_t budget) {
-                int st = ib == 2 ? 2 : 3;
-                while (st >= 2 && stream_smem(nt, ib, warps, st, m, per, c) > budget) st--;
-                return st;
-            };
-            int warps = 8, stages = fit(8, kSmemPerSM / 2 - 1024);  // two CTAs of 8 warps an SM
-            if (stages < 2) stages = fit(warps = 16, max_smem);      // one of 16
-            if (stages < 2) stages = fit(warps = 8, max_smem);       // or of 8
-            if (stages < 2) continue;
-            s.tokens = m;
-            s.nt = nt;
-            s.ib = ib;
-            s.nch = nch;
-            s.cluster = c;
-            s.per = per;
-            s.warps = warps;
-            s.stages = stages;
-        }
-    }
-    if (!s.tokens) return s;
-    s.wk = s.warps;
-    if (s.cluster == 1) {
-        const int slots = num_sms * 16;
-        double best = 1e30;
-        for (int wk = 1; wk <= s.warps; wk *= 2) {
-            const double cost = (double)(((long long)tiles * wk + slots - 1) / slots) * ((s.nch + wk - 1) / wk + (wk == 1 ? 0.5 : 1.0));
-            if (cost < best) best = cost, s.wk = wk;
-        }
+        for (int c = 1; c <= kMaxCluster && !s.tokens; c *= 2)
+            for (int ib = a.K >= 2048 ? 2 : 1; ib >= 1 && !s.tokens; ib--) {
+                const int nch = (int)((a.K + ib * kBoxK - 1) / (ib * kBoxK));
+                const int per = (nch + c - 1) / c;
+                if ((nch + per - 1) / per != c) continue;  // a rank would have nothing
+                // Warps that share a tile: as few as keep every SM's 16 busy.
+                auto share = [&](int warps) {
+                    int wk = warps;
+                    if (c > 1) return wk;
+                    const int slots = num_sms * 16;
+                    double best = 1e30;
+                    for (int k = 1; k <= warps; k *= 2) {
+                        const double cost = (double)(((long long)tiles * k + slots - 1) / slots) * ((nch + k - 1) / k + (k == 1 ? 0.5 : 1.0));
+                        if (cost < best) best = cost, wk = k;
+                    }
+                    return wk;
+                };
+                const int most = ib == 2 ? 2 : 3;
+                auto fit = [&](int warps, int fewest, size_t budget) {
+                    int st = most;
+                    while (st >= fewest && stream_smem(nt, ib, warps, st, m, per, c, share(warps)) > budget) st--;
+                    return st >= fewest ? st : 0;
+                };
+                int warps = 8, stages = fit(8, 2, kSmemPerSM / 2 - 1024);
+                if (!stages) stages = fit(warps = 16, 2, max_smem);
+                if (!stages && ib == 1) stages = fit(warps = 8, 2, max_smem);
+                if (!stages) continue;
+                s.tokens = m;
+                s.nt = nt;
+                s.ib = ib;
+                s.nch = nch;
+                s.cluster = c;
+                s.per = per;
+                s.warps = warps;
+                s.stages = stages;
+                s.wk = share(warps);
+            }
     }
     return s;
 }
