@@ -325,17 +325,27 @@ __device__ __noinline__ void read_lists(const Row<IT, OT, C> r, int mine, const 
         list[atomicAdd(listed, 1)] = (typename S::Listed)u;
         atomicOr(bits + (u >> 5), 1u << (u & 31));
     };
-    for (int j0 = tid; j0 < hlen; j0 += 8 * kThreads) {
-        int id[8];
+    // Eight ids on their way where the history is long; two where it is short, since fetching the code of
+    // eight takes longer than their loads do (200 ids: 6.5 us, with eight 6.7; 4096 ids in 64 rows: 27 us, with four 29).
+    auto count_ids = [&](auto width) {
+        constexpr int U = decltype(width)::value;
+#pragma unroll 1
+        for (int j0 = tid; j0 < hlen; j0 += U * kThreads) {
+            int id[U];
 #pragma unroll
-        for (int i = 0; i < 8; i++) id[i] = j0 + i * kThreads < hlen ? __ldg(hist + j0 + i * kThreads) : -1;
-        if (j0 == tid && k0 == 0) request();
+            for (int i = 0; i < U; i++) id[i] = j0 + i * kThreads < hlen ? __ldg(hist + j0 + i * kThreads) : -1;
+            if (j0 == tid && k0 == 0) request();
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            r.with_slot(id[i], k0, room, [&](int u) {
-                if (j0 + i * kThreads < plen ? S::mark(count, u) : S::add(count, u)) name(u);
-            });
-    }
+            for (int i = 0; i < U; i++)
+                r.with_slot(id[i], k0, room, [&](int u) {
+                    if (j0 + i * kThreads < plen ? S::mark(count, u) : S::add(count, u)) name(u);
+                });
+        }
+    };
+    if (hlen <= 2 * kThreads)
+        count_ids(std::integral_constant<int, 2>());
+    else
+        count_ids(std::integral_constant<int, 8>());
     if (blen) {
         for (int j = tid; j < blen; j += kThreads)
             r.with_slot(__ldg(bids + j), k0, room, [&](int u) { S::raise(entry, u, (uint32_t)(j + 1)); });
