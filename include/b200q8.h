@@ -271,8 +271,16 @@ B200Q8_API int b200q8_quantize_q4_bf16(const uint16_t* w, size_t N, size_t K, in
 B200Q8_API int b200q8_dequantize_q4(void* out, int out_dtype, const uint8_t* q4, const uint16_t* scales, int group,
                                     const int32_t* rows, size_t R, size_t N, size_t K, b200q8_stream_t stream);
 
-/* out[M, N] = inp[M, K] . w[N, K]^T + bias[N]; bias may be NULL.  inp and out are fp32 or fp16;
- * products are exact and sums fp32, whatever the types.  inp must not overlap out. */
+/* out[M, N] = inp[M, K] . w[N, K]^T + bias[N]; bias may be NULL.  inp and out are fp32 or fp16; any M.
+ * Weights are used as they are, q * s with all its bits, and sums are fp32, whatever the types.  What is rounded
+ * before them: at up to 8 tokens (16 for some shapes; fp32 inputs at any number) an input to 2^-23
+ * of the largest |inp| of its 128 consecutive ones (none below counts finer than 2^-122); above, with
+ * fp16 inputs, a scale below 2^-29 of its row's largest.  Scales' magnitudes are to be below 2^90.
+ * An infinity or NaN in inp reaches its own row of out only, as the formula has it.
+ * K a multiple of 32 with inp and q4 16-byte and scales 4-byte aligned is fast; the rest is correct.
+ * fp16 calls of more than 8 tokens share a scratch per stream, allocated (cudaMalloc) with the first such
+ * call and kept.  Captured into a graph they get scratch of the graph's own, also where
+ * it is the stream's first call: graphs may be replayed on any streams, beside each other. */
 B200Q8_API int b200q8_linear_q4(void* out, int out_dtype, const void* inp, int in_dtype, const uint8_t* q4,
                                 const uint16_t* scales, int group, const float* bias, size_t M, size_t N, size_t K,
                                 b200q8_stream_t stream);
@@ -319,7 +327,7 @@ typedef struct b200q8_logit_rules {
  * out may be NULL (only the tokens are wanted), or logits itself (same type and stride); it must not
  * overlap logits otherwise.  argmax (int32 [M]) may be NULL.  rules may be NULL.  Token ids outside
  * [0, V) in the lists are ignored; lengths are clamped to [0, history_count] and [0, bias_count].
- * One launch, no scratch. */
+ * Each operation is IEEE's, also where a penalty is 0, negative, infinite or NaN.  One launch, no scratch. */
 B200Q8_API int b200q8_process_logits(void* out, int out_dtype, size_t out_stride, const void* logits, int in_dtype,
                                      size_t in_stride, size_t M, size_t V, const b200q8_logit_rules* rules,
                                      int32_t* argmax, b200q8_stream_t stream);

@@ -183,25 +183,60 @@ def test_a_graph_outlives_a_larger_call_on_its_stream(cuda):
     assert np.array_equal(out.cpu().numpy(), want) and np.array_equal(o2.cpu().numpy(), big[3])
 
 
-def test_a_first_call_inside_a_capture_is_refused_where_it_needs_scratch(cuda):
-    """The GEMM allocates with its first call on a stream: refused in a capture, which goes on unharmed."""
+def test_graphs_of_one_stream_run_beside_each_other_and_beside_its_calls(cuda):
+    """Graphs captured on one stream (the first calls there, so what they need is allocated during the captures)
+    keep scratch of their own: replayed on other streams at once, beside calls on the stream of the capture."""
     import torch
 
     import vvllm_b200 as v
 
-    st = torch.cuda.Stream()
-    x, q4, sc, want = _linear_inputs(cuda, 40, 300, 256, 11)
-    out, small = torch.zeros((40, 300), device=cuda), torch.zeros((1, 300), device=cuda)
+    st, others = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(3)]
+    for again in range(3):  # graphs before are gone: their scratch is taken again
+        jobs = [(*_linear_inputs(cuda, M, 2000, K, 60 + i), torch.empty((M, 2000), device=cuda))
+                for i, (M, K) in enumerate([(40, 1024), (300, 2048), (40, 1024), (33, 4096)])]
+        small = torch.empty((2, 2000), device=cuda)
+        torch.cuda.synchronize()
+        graphs = []
+        for x, q4, sc, _, out in jobs[:3]:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                v.linear_q4(out, x, q4, sc, 64, stream=st)
+                v.linear_q4(small, x[:2], q4, sc, 64, stream=st)
+                v.linear_q4(out, x, q4, sc, 64, stream=st)
+            graphs.append(g)
+        for _ in range(30):
+            for g, o in zip(graphs, others):
+                with torch.cuda.stream(o):
+                    g.replay()
+            x, q4, sc, _, out = jobs[3]
+            v.linear_q4(out, x, q4, sc, 64, stream=st)
+        torch.cuda.synchronize()
+        for x, q4, sc, want, out in jobs:
+            assert np.array_equal(out.cpu().numpy(), want)
+            out.fill_(float("nan"))
+        del graphs, g
+
+
+def test_two_branches_of_one_capture(cuda):
+    """Calls on two streams of one capture run beside each other in the graph."""
+    import torch
+
+    import vvllm_b200 as v
+
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    jobs = [(*_linear_inputs(cuda, 40, 2000, 2048, 80 + i), torch.empty((40, 2000), device=cuda)) for i in range(2)]
     torch.cuda.synchronize()
     g = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g, stream=st):
-        with pytest.raises(v.B200Q8Error, match="before the capture") as e:
-            v.linear_q4(out, x, q4, sc, 64, stream=st)
-        assert e.value.status == -6
-        v.linear_q4(small, x[:1], q4, sc, 64, stream=st)  # no scratch: captured
-    g.replay()
+    with torch.cuda.graph(g, stream=a):
+        b.wait_stream(a)
+        for (x, q4, sc, _, out), s in zip(jobs, (a, b)):
+            v.linear_q4(out, x, q4, sc, 64, stream=s)
+        a.wait_stream(b)
+    for _ in range(20):
+        g.replay()
     torch.cuda.synchronize()
-    assert np.array_equal(small.cpu().numpy(), want[:1])
+    for x, q4, sc, want, out in jobs:
+        assert np.array_equal(out.cpu().numpy(), want)
 
 
 def test_weights_used_right_after_they_are_written(cuda):

@@ -138,22 +138,13 @@ int grow(T** buf, size_t* have, size_t need, size_t dflt, cudaStream_t stream, b
     return B200Q8_OK;
 }
 
-// capture_ok false: a call that would have to allocate during a capture is refused (the allocation would
-// end the capture) instead of attempted.
-int get_scratch(const ScratchNeed& need, int num_sms, cudaStream_t stream, TcScratch* out, bool capture_ok = true)
+int get_scratch(const ScratchNeed& need, int num_sms, cudaStream_t stream, TcScratch* out)
 {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
     std::lock_guard<std::mutex> lk(g_scratch_mu);
     TcScratch& s = g_scratch[ScratchKey{dev, stream}];
-    if (!capture_ok && (s.ws_floats < need.ws || s.counters < need.counters || s.act_bytes < need.act)) {
-        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess) cudaGetLastError();
-        if (capture != cudaStreamCaptureStatusNone)
-            return fail(B200Q8_ERR_ALLOC, "this call would have to allocate scratch, which a stream capture does not "
-                        "allow: make a call of the same shape on this stream before the capture");
-    }
     // Default capacities: 128-column partials on every SM, 64K tiles.
     int st;
     if ((st = grow(&s.ws, &s.ws_floats, need.ws, (size_t)2 * num_sms * 128 * 128, stream, false, "partials")) ||
@@ -170,9 +161,129 @@ int get_scratch(const ScratchNeed& need, int num_sms, cudaStream_t stream, TcScr
     return B200Q8_OK;
 }
 
+// Scratch of calls captured into a graph: the graph's own, so that its replays may run beside other calls
+// on the stream of the capture and beside other graphs.  One set per (capture, stream), held by the
+// graph (and what is instantiated from it) through a user object; when the last of them is destroyed the
+// set goes back to be taken by a later capture.  Never destroyed, as graphs may outlive this library's statics.
+struct CaptureScratch {
+    int dev = 0;
+    bool taken = false;
+    unsigned long long capture = 0;  // whose calls on `stream` it serves
+    cudaStream_t stream = nullptr;
+    TcScratch s;
+};
+std::mutex& g_capture_mu = *new std::mutex;  // not held during CUDA calls: a release may come from within one
+std::vector<CaptureScratch*>& g_capture = *new std::vector<CaptureScratch*>;
+
+void CUDART_CB release_capture_scratch(void* p)  // may not call CUDA
+{
+    std::lock_guard<std::mutex> lk(g_capture_mu);
+    static_cast<CaptureScratch*>(p)->taken = false;
+}
+
+bool holds(const TcScratch& s, const ScratchNeed& need)
+{
+    return s.ws_floats >= need.ws && s.counters >= need.counters && s.act_bytes >= need.act;
+}
+
+// Allocates during a capture, which goes on: this thread's calls are let through, and the counters are
+// zeroed on a stream of their own.
+int fill_capture_scratch(const ScratchNeed& need, bool fresh, TcScratch* s)
+{
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaThreadExchangeStreamCaptureMode");
+    cudaStream_t own = nullptr;
+    int st = B200Q8_OK;
+    if ((e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking)) != cudaSuccess) st = cuda_fail(e, "cudaStreamCreate");
+    if (!st && fresh &&
+        ((st = grow(&s->ws, &s->ws_floats, need.ws, 0, own, false, "partials")) ||
+         (st = grow(&s->counter_ptr, &s->counters, need.counters, (size_t)1 << 12, own, false, "counters")) ||
+         (st = grow(&s->act, &s->act_bytes, need.act, 0, own, false, "scales")))) {
+        cudaFree(s->ws);
+        cudaFree(s->counter_ptr);
+    }
+    if (!st && (e = cudaMemsetAsync(s->counter_ptr, 0, s->counters * sizeof(int), own)) != cudaSuccess)
+        st = cuda_fail(e, "scratch memset");
+    if (!st && (e = cudaStreamSynchronize(own)) != cudaSuccess) st = cuda_fail(e, "scratch memset");
+    if (own) cudaStreamDestroy(own);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return st;
+}
+
+int capture_scratch(ScratchNeed need, int dev, cudaStream_t stream, unsigned long long capture, cudaGraph_t graph,
+                    TcScratch* out)
+{
+    // In powers of two, so that a later capture finds one that fits.
+    for (size_t* n : {&need.ws, &need.counters, &need.act}) {
+        size_t up = 1024;
+        while (up < *n) up *= 2;
+        *n = up;
+    }
+    CaptureScratch* c = nullptr;
+    {
+        std::lock_guard<std::mutex> lk(g_capture_mu);
+        for (CaptureScratch* i : g_capture) {
+            if (i->dev != dev || !holds(i->s, need)) continue;
+            if (i->taken && i->capture == capture && i->stream == stream) {
+                *out = i->s;
+                return B200Q8_OK;
+            }
+            if (!i->taken && (!c || i->s.ws_floats < c->s.ws_floats)) c = i;
+        }
+        if (c) {
+            c->taken = true;
+            c->capture = capture;
+            c->stream = stream;
+        }
+    }
+    const bool fresh = !c;
+    if (fresh) {
+        c = new CaptureScratch;
+        c->dev = dev;
+        c->taken = true;
+        c->capture = capture;
+        c->stream = stream;
+    }
+    const int st = fill_capture_scratch(need, fresh, &c->s);
+    if (st) {
+        if (fresh)
+            delete c;
+        else
+            release_capture_scratch(c);
+        return st;
+    }
+    if (fresh) {
+        std::lock_guard<std::mutex> lk(g_capture_mu);
+        g_capture.push_back(c);
+    }
+    cudaUserObject_t held = nullptr;
+    cudaError_t e = cudaUserObjectCreate(&held, c, release_capture_scratch, 1, cudaUserObjectNoDestructorSync);
+    if (e != cudaSuccess) {
+        release_capture_scratch(c);
+        return cuda_fail(e, "cudaUserObjectCreate");
+    }
+    if ((e = cudaGraphRetainUserObject(graph, held, 1, cudaGraphUserObjectMove)) != cudaSuccess) {
+        cudaUserObjectRelease(held, 1);  // releases c
+        return cuda_fail(e, "cudaGraphRetainUserObject");
+    }
+    *out = c->s;
+    return B200Q8_OK;
+}
+
 // After a bounded wait gave up, tile counters may be left non-zero: reset them.
 int reset_scratch_counters(int dev)
 {
+    std::vector<TcScratch> captured;
+    {
+        std::lock_guard<std::mutex> lk(g_capture_mu);
+        for (const CaptureScratch* c : g_capture)
+            if (c->dev == dev) captured.push_back(c->s);
+    }
+    for (const TcScratch& s : captured) {
+        const cudaError_t e = cudaMemset(s.counter_ptr, 0, s.counters * sizeof(int));
+        if (e != cudaSuccess) return cuda_fail(e, "reset scratch counters");
+    }
     std::lock_guard<std::mutex> lk(g_scratch_mu);
     for (auto& kv : g_scratch) {
         if (kv.first.dev != dev) continue;
@@ -345,7 +456,16 @@ int stream_scratch(size_t ws_floats, size_t counters, size_t act_bytes, int num_
     need.ws = ws_floats;
     need.counters = counters;
     need.act = act_bytes;
-    return get_scratch(need, num_sms, stream, out, false);
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long capture = 0;
+    cudaGraph_t graph = nullptr;
+    cudaError_t e = cudaStreamGetCaptureInfo_v2(stream, &status, &capture, &graph, nullptr, nullptr);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaStreamGetCaptureInfo");
+    if (status == cudaStreamCaptureStatusNone) return get_scratch(need, num_sms, stream, out);
+    if (status != cudaStreamCaptureStatusActive) return cuda_fail(cudaErrorStreamCaptureInvalidated, "stream capture");
+    int dev = 0;
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+    return capture_scratch(need, dev, stream, capture, graph, out);
 }
 
 int current_device(int* num_sms, size_t* max_smem)

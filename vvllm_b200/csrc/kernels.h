@@ -172,8 +172,8 @@ struct Q4Args {
 };
 // Any shape and alignment.
 cudaError_t launch_q4_linear_generic(const Q4Args& a, cudaStream_t stream);
-// Streaming tensor-core kernel: K % 32 == 0, q4 and x 16-byte, scales 4-byte aligned.  Any M, in groups of
-// up to 32 (fp16) or 10 (fp32) tokens.  cudaErrorNotSupported: alignment, or K beyond its shared memory.
+// Streaming tensor-core kernel: K % 32 == 0, q4 and x 16-byte, scales 4-byte aligned.  Any M, in passes of
+// up to 8 tokens.  cudaErrorNotSupported: alignment, or K beyond its shared memory.
 bool q4_stream_supports(const Q4Args& a);
 cudaError_t launch_q4_stream(const Q4Args& a, int num_sms, size_t max_smem, cudaStream_t stream);
 
@@ -222,7 +222,8 @@ cudaError_t launch_gather_permute(const void* src, void* dst, int elem_bytes, si
 cudaError_t launch_prologue(int pro, const void* x, void* out, int dtype, const float* norm_w, float eps, size_t M,
                             size_t K, bool pdl, cudaStream_t stream);
 
-// The scratch of (current device, stream), grown to the sizes given; a status.
+// Scratch of the sizes given for a call on the stream: that of (current device, stream), or, during a capture, the
+// captured graph's own; a status.
 int stream_scratch(size_t ws_floats, size_t counters, size_t act_bytes, int num_sms, cudaStream_t stream, TcScratch* out);
 
 // SM count and opt-in shared memory of the current device, as a status (B200Q8_ERR_UNSUPPORTED: not sm_100).
