@@ -300,38 +300,73 @@ def _float_code(name: str, what: str, t) -> int:
 def quantize_q4(w, q4, scales, group: int, stream=None) -> None:
     """q4[N,ceil(K/2)] uint8, scales[N,ceil(K/group)] bf16 = 4-bit group quantization of w[N,K] fp32
     (element 2j in the low, 2j+1 in the high half of byte j, as q + 8; value q * scale)."""
+    T = _torch or _t()
     N, K = w.shape
-    _expect("quantize_q4", "w", w, (N, K), _t().float32)
-    _expect_q4("quantize_q4", q4, scales, group, N, K)
-    _same_device("quantize_q4", w, q4, scales)
-    _check(lib().b200q8_quantize_q4(w.data_ptr(), N, K, group, q4.data_ptr(), scales.data_ptr(), _stream(stream)))
+    if not (w.dtype is T.float32 and w.is_contiguous() and _is_q4(q4, scales, group, N, K, w.get_device())):
+        _quantize_q4_refusal("quantize_q4", w, T.float32, q4, scales, group, N, K)
+    status = (_lib or lib()).b200q8_quantize_q4(w.data_ptr(), N, K, group, q4.data_ptr(), scales.data_ptr(), _stream(stream))
+    if status:
+        _check(status)
 
 
 def quantize_q4_bf16(w, q4, scales, group: int, stream=None) -> None:
     """The same from w[N,K] bfloat16 (or its bits as int16 / uint16)."""
+    T = _torch or _t()
     N, K = w.shape
-    bits = (_t().int16, _t().uint16)
-    _expect("quantize_q4_bf16", "w", w, (N, K), w.dtype if w.dtype in bits else _torch.bfloat16)
-    _expect_q4("quantize_q4_bf16", q4, scales, group, N, K)
-    _same_device("quantize_q4_bf16", w, q4, scales)
-    _check(lib().b200q8_quantize_q4_bf16(w.data_ptr(), N, K, group, q4.data_ptr(), scales.data_ptr(), _stream(stream)))
+    if not (w.dtype in (T.bfloat16, T.int16, T.uint16) and w.is_contiguous()
+            and _is_q4(q4, scales, group, N, K, w.get_device())):
+        _quantize_q4_refusal("quantize_q4_bf16", w, w.dtype if w.dtype in (T.int16, T.uint16) else T.bfloat16, q4, scales,
+                             group, N, K)
+    status = (_lib or lib()).b200q8_quantize_q4_bf16(w.data_ptr(), N, K, group, q4.data_ptr(), scales.data_ptr(),
+                                                     _stream(stream))
+    if status:
+        _check(status)
+
+
+def _is_q4(q4, scales, group, N: int, K: int, dev: int) -> bool:
+    """Whether q4 and scales are a matrix [N, K] on CUDA device dev, the current one."""
+    return (group in _GROUPS and q4.dtype is _torch.uint8 and q4.shape == (N, (K + 1) // 2) and q4.is_contiguous()
+            and scales.dtype is _torch.bfloat16 and scales.shape == (N, -(-K // group)) and scales.is_contiguous()
+            and dev >= 0 and dev == q4.get_device() == scales.get_device() == _torch.cuda.current_device())
+
+
+def _quantize_q4_refusal(name, w, dtype, q4, scales, group, N, K) -> None:
+    _expect(name, "w", w, (N, K), dtype)
+    _expect_q4(name, q4, scales, group, N, K)
+    _same_device(name, w, q4, scales)
+    raise AssertionError("refused without a reason")
 
 
 def dequantize_q4(out, q4, scales, group: int, rows=None, stream=None) -> None:
     """out[R,K] (fp32 or fp16) = values of the rows rows[R] (int32; an index outside the matrix gives
     zeros: the token lookup of a 4-bit embedding), or of all rows."""
+    T = _torch or _t()
     N, (R, K) = q4.shape[0], out.shape
-    _t()
-    _expect_q4("dequantize_q4", q4, scales, group, N, K)
-    _expect("dequantize_q4", "out", out, (R if rows is not None else N, K), out.dtype)
-    code, at = _float_code("dequantize_q4", "out", out), None
+    ot, dev, at = out.dtype, out.get_device(), None
+    if not ((ot is T.float16 or ot is T.float32) and out.is_contiguous() and _is_q4(q4, scales, group, N, K, dev)):
+        _dequantize_q4_refusal(out, q4, scales, group, rows, N, R, K)
     if rows is not None:
-        _expect("dequantize_q4", "rows", rows, (R,), _torch.int32)
+        if not (rows.dtype is T.int32 and rows.shape == (R,) and rows.is_contiguous() and rows.get_device() == dev):
+            _dequantize_q4_refusal(out, q4, scales, group, rows, N, R, K)
         at = rows.data_ptr()
-    _same_device("dequantize_q4", out, q4, scales, rows)
+    elif R != N:
+        _dequantize_q4_refusal(out, q4, scales, group, rows, N, R, K)
     if R:  # (no rows: an empty list has no address)
-        _check(lib().b200q8_dequantize_q4(out.data_ptr(), code, q4.data_ptr(), scales.data_ptr(), group, at, R, N, K,
-                                          _stream(stream)))
+        status = (_lib or lib()).b200q8_dequantize_q4(out.data_ptr(), F16 if ot is T.float16 else F32, q4.data_ptr(),
+                                                      scales.data_ptr(), group, at, R, N, K, _stream(stream))
+        if status:
+            _check(status)
+
+
+def _dequantize_q4_refusal(out, q4, scales, group, rows, N, R, K) -> None:
+    name = "dequantize_q4"
+    _expect_q4(name, q4, scales, group, N, K)
+    _expect(name, "out", out, (R if rows is not None else N, K), out.dtype)
+    _float_code(name, "out", out)
+    if rows is not None:
+        _expect(name, "rows", rows, (R,), _torch.int32)
+    _same_device(name, out, q4, scales, rows)
+    raise AssertionError("refused without a reason")
 
 
 def linear_q4(out, x, q4, scales, group: int, bias=None, stream=None) -> None:
@@ -347,10 +382,10 @@ def linear_q4_add(out, x, q4, scales, group: int, bias, residual, stream=None) -
     xcode, ocode = (F16 if xt is T.float16 else F32), (F16 if ot is T.float16 else F32)
     dev = x.get_device()
     # one pass over what has to hold; _linear_q4_refusal says what does not
-    if not (group in _GROUPS and q4.dtype is T.uint8 and q4.shape == (N, (K + 1) // 2) and q4.is_contiguous()
-            and scales.dtype is T.bfloat16 and scales.shape == (N, -(-K // group)) and scales.is_contiguous()
-            and (xt is T.float16 or xt is T.float32) and x.is_contiguous()
+    if not ((xt is T.float16 or xt is T.float32) and x.is_contiguous()
             and (ot is T.float16 or ot is T.float32) and out.shape == (M, N) and out.is_contiguous()
+            and group in _GROUPS and q4.dtype is T.uint8 and q4.shape == (N, (K + 1) // 2) and q4.is_contiguous()
+            and scales.dtype is T.bfloat16 and scales.shape == (N, -(-K // group)) and scales.is_contiguous()
             and dev >= 0 and dev == out.get_device() == q4.get_device() == scales.get_device() == T.cuda.current_device()):
         _linear_q4_refusal(out, x, q4, scales, group, bias, residual, M, N, K)
     b = r = None
@@ -391,9 +426,11 @@ class _LogitRules(ctypes.Structure):
                 ("allowed_stride", _sz)]
 
 
-def _rows_of(name: str, what: str, t, M: int, dtype):
-    """(address, row stride, columns) of t: [M, n] with contiguous rows, or [n] / [1, n] shared by all rows
+def _rows_of(name: str, what: str, t, M: int, dtype, dev: int):
+    """(address, row stride, columns) of t on device dev: [M, n] with contiguous rows, or [n] / [1, n] shared by all rows
     (stride 0).  No columns: no address."""
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: the logits lie on device {dev}, {what} on {t.device}")
     shape = t.shape
     n = shape[-1] if shape else 0
     if len(shape) == 2 and shape[0] == M and t.dtype is dtype and t.is_contiguous():
@@ -407,11 +444,12 @@ def _rows_of(name: str, what: str, t, M: int, dtype):
     return t.data_ptr() or None, stride, n
 
 
-def _per_row(name: str, what: str, t, M: int, dtype):
+def _per_row(name: str, what: str, t, rows: tuple, dtype, dev: int):
     if t is None:
         return None
-    if t.dtype is not dtype or t.shape != (M,) or not t.is_contiguous():
-        _expect(name, what, t, (M,), dtype)
+    if t.dtype is not dtype or t.shape != rows or t.get_device() != dev or not t.is_contiguous():
+        _expect(name, what, t, rows, dtype)
+        raise ValueError(f"{name}: the logits lie on device {dev}, {what} on {t.device}")
     return t.data_ptr()
 
 
@@ -424,44 +462,51 @@ def process_logits(out, logits, argmax=None, history=None, history_len=None, pro
     out: fp32 or fp16, logits itself, or None.  history / bias_ids / bias_values / allowed: [M, n]
     int32 / int32 / fp32 / int32 (bit i % 32 of word i // 32), or one row for all; the other rules are
     [M]: int32 lengths and fp32 penalties.  Rows of every 2-D tensor are contiguous, any row stride."""
-    name = "process_logits"
+    name, T = "process_logits", _torch or _t()
     M, V = logits.shape
-    i32, f32 = _t().int32, _torch.float32
-    xs = logits.stride()
-    os_ = xs if out is logits or out is None else out.stride()
-    if V > 1 and (xs[1] != 1 or os_[-1] != 1) or (out is not None and out.shape != (M, V)):
-        raise ValueError(f"{name}: logits and out must be [{M}, {V}] with contiguous rows")
-    am = _per_row(name, "argmax", argmax, M, i32)
+    i32, f32, per = T.int32, T.float32, (M,)
+    xt, xs, dev = logits.dtype, logits.stride(), logits.get_device()
+    if out is None or out is logits:
+        to, ot, os_ = None if out is None else logits.data_ptr(), xt, xs
+    else:
+        to, ot, os_ = out.data_ptr(), out.dtype, out.stride()
+        if out.shape != (M, V):
+            raise ValueError(f"{name}: out must be [{M}, {V}] with contiguous rows, got {list(out.shape)}")
+        if out.get_device() != dev:
+            _same_device(name, logits, out)
+    if V > 1 and (xs[1] != 1 or os_[1] != 1):
+        raise ValueError(f"{name}: logits and out must have contiguous rows")
+    if not ((xt is T.float16 or xt is f32) and (ot is T.float16 or ot is f32)):
+        _float_code(name, "logits", logits)
+        _float_code(name, "out", out)
+    am = _per_row(name, "argmax", argmax, per, i32, dev)
     rules = None
-    hist = bids = bvals = mask = None
     if history is not None or bias_ids is not None or bias_values is not None or allowed is not None:
+        hist = bids = bvals = mask = None
         hstride = hcount = bstride = bcount = mstride = 0
         if history is not None:
-            hist, hstride, hcount = _rows_of(name, "history", history, M, i32)
+            hist, hstride, hcount = _rows_of(name, "history", history, M, i32, dev)
         if bias_ids is not None:
-            bids, bstride, bcount = _rows_of(name, "bias_ids", bias_ids, M, i32)
+            bids, bstride, bcount = _rows_of(name, "bias_ids", bias_ids, M, i32, dev)
         if bias_values is not None:
-            bvals, vstride, vcount = _rows_of(name, "bias_values", bias_values, M, f32)
+            bvals, vstride, vcount = _rows_of(name, "bias_values", bias_values, M, f32, dev)
             if bias_ids is None or (vstride, vcount) != (bstride, bcount):
                 raise ValueError(f"{name}: bias_values must be laid out like bias_ids")
         if allowed is not None:
-            mask, mstride, words = _rows_of(name, "allowed", allowed, M, i32)
+            mask, mstride, words = _rows_of(name, "allowed", allowed, M, i32, dev)
             if words < (V + 31) // 32:
                 raise ValueError(f"{name}: allowed needs {(V + 31) // 32} words a row, got {words}")
-        rules = _LogitRules(hist, hstride, hcount, _per_row(name, "history_len", history_len, M, i32),
-                            _per_row(name, "prompt_len", prompt_len, M, i32),
-                            _per_row(name, "repetition", repetition, M, f32), _per_row(name, "presence", presence, M, f32),
-                            _per_row(name, "frequency", frequency, M, f32), bids, bvals, bstride, bcount,
-                            _per_row(name, "bias_len", bias_len, M, i32), mask, mstride)
-    _same_device(name, logits, out, argmax, history, history_len, prompt_len, repetition, presence, frequency, bias_ids,
-                 bias_values, bias_len, allowed)
-    xcode = _float_code(name, "logits", logits)
-    if out is None:
-        to, ocode, ostride = None, xcode, V
-    else:
-        to, ocode, ostride = out.data_ptr(), _float_code(name, "out", out), os_[0] if M > 1 else V
-    status = (_lib or lib()).b200q8_process_logits(to, ocode, ostride, logits.data_ptr(), xcode, xs[0] if M > 1 else V, M, V,
-                                                   None if rules is None else ctypes.addressof(rules), am, _stream(stream))
+        rules = _LogitRules(hist, hstride, hcount, _per_row(name, "history_len", history_len, per, i32, dev),
+                            _per_row(name, "prompt_len", prompt_len, per, i32, dev),
+                            _per_row(name, "repetition", repetition, per, f32, dev),
+                            _per_row(name, "presence", presence, per, f32, dev),
+                            _per_row(name, "frequency", frequency, per, f32, dev), bids, bvals, bstride, bcount,
+                            _per_row(name, "bias_len", bias_len, per, i32, dev), mask, mstride)
+    if dev < 0 or dev != T.cuda.current_device():
+        _same_device(name, logits)
+    status = (_lib or lib()).b200q8_process_logits(
+        to, F16 if ot is T.float16 else F32, os_[0] if M > 1 else V, logits.data_ptr(), F16 if xt is T.float16 else F32,
+        xs[0] if M > 1 else V, M, V, None if rules is None else ctypes.addressof(rules), am, _stream(stream))
     if status:
         _check(status)
 

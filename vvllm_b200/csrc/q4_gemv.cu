@@ -88,8 +88,8 @@ cudaError_t launch_generic(const Q4Args& a, cudaStream_t stream)
 // X = 65536 X2 + 256 X1 + X0: three columns of the product.  The codes become bytes 16 q with three
 // integer operations per eight (one shift, two and-xor).  So mma.sync m16n8k32 (s8) sums 16 q * Xd
 // of a group exactly, and in fp32 every group's sum is multiplied by the group's scale and the
-// chunk's power of two and added to the row's.  What is rounded: an element to 2^-23 of its chunk's
-// largest (fp16 tokens are exact down to 2^-12 of it), and the fp32 sums, once a group.  A chunk that
+// chunk's power of two and added to the row's.  What is rounded: an element, by at most 2^-22 of its
+// chunk's largest (fp16 tokens are exact down to 2^-11 of it), and the fp32 sums, once a group.  A chunk that
 // holds an infinity or NaN is summed directly instead.  Chunks below 2^-100 count as below 2^-100.
 //
 // Why not fp16 operands: unpacking to fp16 takes 18 operations per 16 x 32 weights and two products,
