@@ -439,51 +439,50 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
             tc::tma_load_2d_hint(ring + stage * kItemBytes + b * kBoxBytes, &tmW, (ich * IB + b) * 128, itile * 16,
                                  bar0 + 8 * stage, policy);
     };
-    // Scales, two to a word, of the box about to be multiplied and of the next; those of the one after are
-    // loaded meanwhile (a box takes less than a load from L2).
+    // Scales, two to a word, of the item about to be multiplied; those of the next (with items of one box, of
+    // the two next) are loaded meanwhile: a box takes less than a load from L2.
     constexpr int kSW = kBoxGroups / 2;
     struct Scales {
-        uint32_t a[kSW], b[kSW];  // the fragment's two rows
+        uint32_t a[IB][kSW], b[IB][kSW];  // the fragment's two rows
     };
-    int stile = busy ? tile0 : p.tiles, sch = ch0 + kw, sbox = 0;  // the box whose scales are loaded next
+    int stile = busy ? tile0 : p.tiles, sch = ch0 + kw;  // the item whose scales are loaded next
     const uint16_t* sp = nullptr;
     size_t srow = 0;  // from the first row's scales to the other's
-    const bool swide = ng % kBoxGroups == 0 && ((uintptr_t)p.a.scales & (2 * kBoxGroups - 1)) == 0;  // one load a row
+    const bool swide = ng % kBoxGroups == 0 && ((uintptr_t)p.a.scales & (2 * kBoxGroups - 1)) == 0;  // one load a row and box
     auto load_scales = [&](Scales& s) {
         if (stile >= p.tiles) return;
-        if (sbox == 0 && sch == ch0 + kw) {
+        if (sch == ch0 + kw) {
             const int n0 = min(stile * 16 + row, N - 1), n1 = min(stile * 16 + row + 8, N - 1);
             sp = p.a.scales + (size_t)n0 * ng + sch * IB * kBoxGroups;
             srow = (size_t)(n1 - n0) * ng;
         }
-        const int g0 = (sch * IB + sbox) * kBoxGroups;
-        if (swide) {
-            if (g0 < ng) {
-                load_words(sp, s.a);
-                load_words(sp + srow, s.b);
+        const int left = ng - sch * IB * kBoxGroups;  // groups from here to the row's end
+#pragma unroll
+        for (int b = 0; b < IB; b++) {
+            if (swide) {
+                if (b * kBoxGroups < left) {
+                    load_words(sp + b * kBoxGroups, s.a[b]);
+                    load_words(sp + srow + b * kBoxGroups, s.b[b]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kSW; i++) s.a[b][i] = s.b[b][i] = 0;
+                }
             } else {
 #pragma unroll
-                for (int i = 0; i < kSW; i++) s.a[i] = s.b[i] = 0;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kBoxGroups; i++) {
-                const bool in = g0 + i < ng;  // a row's last box may be short
-                const uint32_t a = in ? (uint32_t)__ldg(sp + i) : 0u, b = in ? (uint32_t)__ldg(sp + srow + i) : 0u;
-                s.a[i / 2] = i & 1 ? s.a[i / 2] | a << 16 : a;
-                s.b[i / 2] = i & 1 ? s.b[i / 2] | b << 16 : b;
+                for (int i = 0; i < kBoxGroups; i++) {
+                    const int j = b * kBoxGroups + i;
+                    const bool in = j < left;  // a row's last box may be short
+                    const uint32_t x = in ? (uint32_t)__ldg(sp + j) : 0u, y = in ? (uint32_t)__ldg(sp + srow + j) : 0u;
+                    s.a[b][i / 2] = i & 1 ? s.a[b][i / 2] | x << 16 : x;
+                    s.b[b][i / 2] = i & 1 ? s.b[b][i / 2] | y << 16 : y;
+                }
             }
         }
-        if (++sbox < IB) {
-            sp += kBoxGroups;
-        } else {
-            sbox = 0;
-            sch += wk;
-            sp += ((wk - 1) * IB + 1) * kBoxGroups;
-            if (sch >= ch1) {
-                sch = ch0 + kw;
-                stile += tstep;
-            }
+        sch += wk;
+        sp += wk * IB * kBoxGroups;
+        if (sch >= ch1) {
+            sch = ch0 + kw;
+            stile += tstep;
         }
     };
     Scales sc{}, sc_next{};
@@ -497,7 +496,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
             advance();
         }
         load_scales(sc);
-        load_scales(sc_next);
+        if (IB == 1) load_scales(sc_next);
     };
     auto arrived = [&]() {
         if (lane == 0)
@@ -539,10 +538,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
             uint32_t xitem = (uint32_t)(ch - ch0) * (C::kChunks * 128);
             const float* wchunk = weight + (ch - ch0) * C::kChunks * C::kCols + 2 * t;
             // Chunks behind K need no care: their codes and tokens are zeros, and so are their scales.
-#pragma unroll 1
+            Scales sc_after = sc;
+            load_scales(sc_after);
+#pragma unroll
             for (int box = 0; box < IB; box++) {
-                Scales sc_after = sc_next;
-                load_scales(sc_after);
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     uint32_t x[NT][2][4];
@@ -576,7 +575,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
                         const int si = c * GC + gi;
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            const uint32_t word = i == 0 ? sc.a[si / 2] : sc.b[si / 2];
+                            const uint32_t word = i == 0 ? sc.a[box][si / 2] : sc.b[box][si / 2];
                             const float r = __uint_as_float(si & 1 ? word & 0xFFFF0000u : word << 16);
                             float2 f = tile_value(d[0], i);
                             if constexpr (NT == 3)  // X0 + 256 X1 + 65536 X2
@@ -589,12 +588,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
                     acc[0] = __ffma2_rn(sum[0], wt, acc[0]);
                     acc[1] = __ffma2_rn(sum[1], wt, acc[1]);
                 }
-                sc = sc_next;
-                sc_next = sc_after;
                 wrow += kBoxBytes;
                 xitem += 256;
                 wchunk += 2 * C::kCols;
             }
+            sc = IB == 1 ? sc_next : sc_after;
+            sc_next = sc_after;
             fence(acc[0].x), fence(acc[0].y), fence(acc[1].x), fence(acc[1].y);
             __syncwarp();  // the stage is read
             if (ok) {  // else the ring stays as it is, for the end
