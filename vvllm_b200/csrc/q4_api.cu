@@ -97,9 +97,9 @@ int linear_q4(const char* what, void* out, int out_dtype, const void* inp, int i
     a.out_dtype = out_dtype;
     // Up to 8 tokens the streaming kernel reads the weights once; above, once for every 8, where the GEMM
     // (fp16 tokens) reads them once at a rate bound by its dequantization.  Measured on B200, streaming vs GEMM:
-    // 37888 x 3584 at 8 tokens 23 vs 37 us, at 9 37 vs 38, at 16 46 vs 38; 3584 x 18944 at 8 33 vs 28, at 16 65 vs 28.
+    // 37888 x 3584 at 8 tokens 22 vs 37 us, at 9 36 vs 38, at 16 45 vs 38; 3584 x 18944 at 8 25 vs 28, at 16 49 vs 28.
     // For 9 to 16 tokens and few weights with a long K, of which the GEMM makes few tiles, two passes still
-    // win: 3584 x 3584 at 16 19 vs 19, 896 x 4864 23 vs 24, 512 x 18944 29 vs 32; not 4864 x 896, 14 vs 10.
+    // win: 3584 x 3584 at 16 19 vs 19, 896 x 4864 19 vs 24, 512 x 18944 28 vs 32; not 4864 x 896, 14 vs 10.
     const bool gemm = M > 16 || (M > 8 && (N * K > ((size_t)1 << 24) || K < 2048));
     cudaError_t e;
     if (gemm && q4_gemm_tc_supports(a)) {

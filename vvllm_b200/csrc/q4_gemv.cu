@@ -93,12 +93,15 @@ cudaError_t launch_generic(const Q4Args& a, cudaStream_t stream)
 // holds an infinity or NaN is summed directly instead.  Chunks below 2^-100 count as below 2^-100.
 //
 // Why not fp16 operands: unpacking to fp16 takes 18 operations per 16 x 32 weights and two products,
-// to bytes 6 and one; on B200 (gate/up of a 7B model, 37888 x 3584, one token) the fp16 form of this
-// kernel ran at 17.9 us, bound by instruction issue.  Why not tcgen05: its operands would have to be
+// to bytes 6 and one; for one token and 37888 x 3584 the fp16 form of this kernel ran at 17.9 us,
+// bound by instruction issue, where this one takes 13.4.  Why not tcgen05: its operands would have to be
 // written back to shared or tensor memory as bytes, twice what was read; at 8 cycles a product, one
 // per three columns of 16 x 32 weights, mma.sync is within what HBM allows (about 44 cycles) to 13 tokens.
 //
-// Bound by HBM: half a byte a weight.
+// Bound by HBM (half a byte a weight) for one and two tokens once there are megabytes to stream: 152064 x 3584
+// at 46 us, 6.1 TB/s; 37888 x 3584 at 13.4 us, of which 3 are start and tokens.  At three to eight tokens by
+// instruction issue and its dependences, 33 instructions a 16 x 32 block: 152064 x 3584 73 us, 37888 x 3584 22 us,
+// at eight; with long K also by the tokens' way into shared memory: 3584 x 18944 12 us at one, 25 at eight.
 //
 // Work: a tile is 16 rows; an item is a tile's next 256 or 512 of K.  `wk` warps share a tile (item ch
 // goes to warp ch mod wk) and add their sums through shared memory in warp order; a CTA of 8 or 16
@@ -360,7 +363,7 @@ struct StreamCfg {
         const int chunks = per * kChunks;
         return 1024 + (size_t)warps * stages * kItemBytes + warps * kMaxStages * 8 + 3 * M * column_stride(chunks * 4) +
                (size_t)chunks * kCols * 4 + (size_t)red_bufs(wk, cluster) * warps * kSums * 4 +
-               (cluster > 1 ? (size_t)2 * cluster * kSums * 4 : 0) + (size_t)M * chunks;
+               (cluster > 1 ? (size_t)2 * cluster * (warps / wk) * kSums * 4 : 0) + (size_t)M * chunks;
     }
 };
 
@@ -387,8 +390,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     const size_t cs = column_stride(xchunks * 4);
     float* weight = reinterpret_cast<float*>(xs + 3 * p.M * cs);
     float* red = weight + xchunks * C::kCols;         // [buffer][warp][tile's outputs]
-    float* cbuf = red + C::red_bufs(p.wk, csize) * warps * C::kSums;  // [2][rank][tile's outputs] of a cluster's CTAs (in rank 0)
-    unsigned char* direct = reinterpret_cast<unsigned char*>(cbuf + (csize > 1 ? 2 * csize * C::kSums : 0));
+    float* cbuf = red + C::red_bufs(p.wk, csize) * warps * C::kSums;  // [2][rank][group][tile's outputs] of a cluster's CTAs (in rank 0)
+    unsigned char* direct = reinterpret_cast<unsigned char*>(cbuf + (csize > 1 ? 2 * csize * (warps >> p.wk_log2) * C::kSums : 0));
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
@@ -488,8 +491,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     Scales sc{}, sc_next{};
 
     // The tokens' loads go first, then one item a warp: behind more they would wait for megabytes to pass (all of
-    // the ring first: 16.5 us for 37888 x 3584 and one token, instead of 14).  Once they are there the ring is
-    // filled, before they are converted.  (Requesting two more items into L2 as well: 14.8 us.)
+    // the ring first: 37888 x 3584, one token, 14.0 us instead of 13.4; 3584 x 18944 13.2, 12.2).  Once they are
+    // there the ring is filled, before they are converted.
     auto asked = [&]() {
         if (lane == 0 && itile < p.tiles) {
             load_item(inflight++);
@@ -524,11 +527,11 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     const int rounds = (p.tiles - tbase + tstep - 1) / tstep;  // uniform in a cluster
     for (int it = 0; it < rounds; it++) {
         const int tile = tile0 + it * tstep;
-        if (tile >= p.tiles) break;  // groups end on their own; with a cluster there is one group
+        if (tile >= p.tiles && csize == 1) break;  // a cluster's groups end together, for its barriers
         if (lane == 0 && kw == 0 && tile + tstep < p.tiles) prefetch_scales(tile + tstep);
         // Of rows row and row + 8: columns 2t and 2t + 1, which are tokens where three tiles hold their bytes.
         float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-        for (int ch = ch0 + kw; ch < ch1; ch += wk) {
+        for (int ch = ch0 + kw; ch < ch1 && tile < p.tiles; ch += wk) {
             if (ok) {
                 ok = __all_sync(0xffffffffu, tc::mbar_wait(bar0 + 8 * stage, phase, &zero, kWaitNs));
                 if (!ok && lane == 0) atomicOr(&g_q4_error, 1);
@@ -634,7 +637,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
                 q4_store<float>(static_cast<float*>(p.a.out) + o, p.a.res ? static_cast<const float*>(p.a.res) + o : nullptr,
                                 y, p.a.bias, n);
         };
-        if (wk == 1 && !any_direct) {
+        if (wk == 1 && csize == 1 && !any_direct) {
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 if (mine(i)) put(mt + (i & 1), row + 8 * (i >> 1), v[i]);
@@ -646,7 +649,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if (mine(i)) wsum[(mt + (i & 1)) * 16 + row + 8 * (i >> 1)] = v[i];
-        if (any_direct) {  // rare: infinities or NaN among this CTA's elements
+        if (any_direct && tile < p.tiles) {  // rare: infinities or NaN among this CTA's elements
             __syncwarp();
             for (int m = 0; m < p.M; m++)
                 for (int c = kw; c < xchunks; c += wk)
@@ -670,16 +673,16 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
             // Rank 0 collects.  The others go on and wait for this tile's barrier before they store for the
             // next: by then rank 0 has read what their buffer held two tiles ago.
             if (it > 0 && rank != 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-            float* to = cluster.map_shared_rank(cbuf, 0) + (parity * csize + rank) * C::kSums;
+            float* to = cluster.map_shared_rank(cbuf, 0) + ((parity * csize + rank) * groups + group) * C::kSums;
             for (int e = gt; e < outs; e += wk * 32) to[e] = warp_sums(e);
             __syncwarp();
             asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
             if (rank == 0) {
                 asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-                const float* from = cbuf + parity * csize * C::kSums;
+                const float* from = cbuf + (parity * csize * groups + group) * C::kSums;
                 for (int e = gt; e < outs; e += wk * 32) {
                     float y = from[e];
-                    for (int c = 1; c < csize; c++) y += from[c * C::kSums + e];
+                    for (int c = 1; c < csize; c++) y += from[c * groups * C::kSums + e];
                     put(e >> 4, e & 15, y);
                 }
                 __syncwarp();
@@ -802,55 +805,59 @@ size_t stream_smem(int nt, int ib, int warps, int stages, int M, int per, int cl
 constexpr int kMaxCluster = 8;
 
 // Items of two boxes where a row has several (a wait, a copy and their bookkeeping cost about as much as a
-// box's products: 37888 x 3584, one token, 15.8 us with one box, 14.9 with two), two items in flight a warp
-// (three: 16.4 us, the copies' queue then holds up the warps); two CTAs of 8 warps an SM where the tokens
-// leave room, else one of 16, else one of 8; a cluster only where one CTA cannot hold the tokens (it measured slower
-// wherever both were possible).
+// box's products: 37888 x 3584, one token, 14.9 us with one box, 13.4 with two), two items in flight a warp
+// (three: 14.4 us, the copies' queue then holds up the warps); sixteen warps an SM, in two CTAs where the
+// tokens leave room, else in one, else in clusters of 2, 4, 8; eight only where that does not fit either
+// (8 tokens, 4096 x 14336: 17 us in clusters of four, with eight warps in clusters of two 26).
+// One or two tokens take a cluster only where one CTA cannot hold them.  With more, putting them into shared memory
+// is what a CTA of few tiles spends its time on, so a long K is split over as many SMs as the tiles
+// leave free (8 tokens, 896 x 4864: 9.2 us on clusters of two, 12 without).
 StreamPlan plan_stream(const Q4Args& a, size_t M, int num_sms, size_t max_smem)
 {
-    StreamPlan s;
-    const int tiles = (int)((a.N + 15) / 16);
-    for (int m = (int)std::min<size_t>(M, kMaxTokens); m >= 1 && !s.tokens; m--) {
+    const long long tiles = (long long)((a.N + 15) / 16);
+    for (int m = (int)std::min<size_t>(M, kMaxTokens); m >= 1; m--) {
         const int nt = m <= 2 ? 1 : 3;
-        for (int c = 1; c <= kMaxCluster && !s.tokens; c *= 2)
-            for (int ib = a.K >= 2048 ? 2 : 1; ib >= 1 && !s.tokens; ib--) {
-                const int nch = (int)((a.K + ib * kBoxK - 1) / (ib * kBoxK));
-                const int per = (nch + c - 1) / c;
-                if ((nch + per - 1) / per != c) continue;  // a rank would have nothing
-                // Warps that share a tile: as few as keep every SM's 16 busy.
-                auto share = [&](int warps) {
-                    int wk = warps;
-                    if (c > 1) return wk;
-                    const int slots = num_sms * 16;
-                    double best = 1e30;
-                    for (int k = 1; k <= warps; k *= 2) {
-                        const double cost = (double)(((long long)tiles * k + slots - 1) / slots) * ((nch + k - 1) / k + (k == 1 ? 0.5 : 1.0));
-                        if (cost < best) best = cost, wk = k;
-                    }
-                    return wk;
-                };
-                const int most = ib == 2 ? 2 : 3;
-                auto fit = [&](int warps, int fewest, size_t budget) {
-                    int st = most;
-                    while (st >= fewest && stream_smem(nt, ib, warps, st, m, per, c, share(warps)) > budget) st--;
-                    return st >= fewest ? st : 0;
-                };
-                int warps = 8, stages = fit(8, 2, kSmemPerSM / 2 - 1024);
-                if (!stages) stages = fit(warps = 16, 2, max_smem);
-                if (!stages && ib == 1) stages = fit(warps = 8, 2, max_smem);
-                if (!stages) continue;
-                s.tokens = m;
-                s.nt = nt;
-                s.ib = ib;
-                s.nch = nch;
-                s.cluster = c;
-                s.per = per;
-                s.warps = warps;
-                s.stages = stages;
-                s.wk = share(warps);
+        int c0 = 1;
+        while (nt == 3 && c0 < kMaxCluster && 2 * c0 * tiles <= num_sms && a.K >= (size_t)4096 * c0) c0 *= 2;
+        for (int all = 1; all >= 0; all--)
+            for (int c = all ? c0 : 1; c <= kMaxCluster; c *= 2) {
+                StreamPlan found;
+                double best = 1e30;  // what a warp has to do, in boxes
+                for (int ib = all && a.K >= 2048 && (nt == 1 || c == 1) ? 2 : 1; ib >= 1; ib--) {
+                    StreamPlan s;
+                    s.tokens = m;
+                    s.nt = nt;
+                    s.ib = ib;
+                    s.cluster = c;
+                    s.nch = (int)((a.K + ib * kBoxK - 1) / (ib * kBoxK));
+                    s.per = (s.nch + c - 1) / c;
+                    if ((s.nch + s.per - 1) / s.per != c) continue;  // a rank would have nothing
+                    // Warps that share a tile (two at least in a cluster, whose rank 0 holds every group's sums): those that
+                    // end soonest, an item costing a third of a box beside its boxes, and the joining of their sums.
+                    auto fit = [&](int warps, size_t budget) {
+                        const long long slots = c == 1 ? num_sms * 16 : num_sms / c * warps;
+                        bool any = false;
+                        s.warps = warps;
+                        for (s.wk = c > 1 ? 2 : 1; s.wk <= warps; s.wk *= 2) {
+                            s.stages = ib == 2 ? 2 : 3;
+                            while (s.stages >= 2 && stream_smem(nt, ib, warps, s.stages, m, s.per, c, s.wk) > budget) s.stages--;
+                            if (s.stages < 2) continue;
+                            any = true;
+                            const double join = c > 1 ? 2.7 : s.wk > 1 ? 1.5 : 0.75;
+                            const double cost = (double)((tiles * s.wk + slots - 1) / slots) * ((s.per + s.wk - 1) / s.wk * (ib + 0.33) + join);
+                            if (cost < best) best = cost, found = s;
+                        }
+                        return any;
+                    };
+                    if (!all)
+                        fit(8, max_smem);
+                    else if (c > 1 || !fit(8, kSmemPerSM / 2 - 1024))
+                        fit(16, max_smem);
+                }
+                if (found.tokens) return found;
             }
     }
-    return s;
+    return StreamPlan{};
 }
 
 }  // namespace
@@ -868,7 +875,8 @@ cudaError_t launch_q4_stream(const Q4Args& a, int num_sms, size_t max_smem, cuda
     const StreamPlan first = plan_stream(a, a.M, num_sms, max_smem);
     if (!first.tokens) return cudaErrorNotSupported;  // one token's slice exceeds the shared memory
     for (size_t m0 = 0; m0 < a.M;) {
-        const StreamPlan s = plan_stream(a, std::min<size_t>(a.M - m0, (size_t)first.tokens), num_sms, max_smem);
+        const size_t left = a.M - m0;
+        const StreamPlan s = left >= (size_t)first.tokens ? first : plan_stream(a, left, num_sms, max_smem);
         StreamParams p;
         p.a = a;
         p.a.x = static_cast<const char*>(a.x) + m0 * a.K * ib;
