@@ -100,7 +100,10 @@ int linear_q4(const char* what, void* out, int out_dtype, const void* inp, int i
     // 37888 x 3584 at 8 tokens 22 vs 37 us, at 9 36 vs 38, at 16 45 vs 38; 3584 x 18944 at 8 25 vs 28, at 16 49 vs 28.
     // For 9 to 16 tokens and few weights with a long K, of which the GEMM makes few tiles, two passes still
     // win: 3584 x 3584 at 16 19 vs 19, 896 x 4864 19 vs 24, 512 x 18944 28 vs 32; not 4864 x 896, 14 vs 10.
-    const bool gemm = M > 16 || (M > 8 && (N * K > ((size_t)1 << 24) || K < 2048));
+    // fp32 outputs take the GEMM only with short sums: the tensor core's accumulator drops what falls below its 24
+    // bits instead of rounding it, 1.8e-8 of the sum per 16 products (512 tokens, K = 18944: 2.2e-5 off, where
+    // fp32 sums in another order are 2e-6 off and the streaming kernel's 3e-7); half an fp16 step is 2^-12.
+    const bool gemm = (M > 16 || (M > 8 && (N * K > ((size_t)1 << 24) || K < 2048))) && (out_dtype == B200Q8_F16 || K <= 512);
     cudaError_t e;
     if (gemm && q4_gemm_tc_supports(a)) {
         size_t ws = 0, counters = 0, act = 0;
