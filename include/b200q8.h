@@ -273,12 +273,12 @@ B200Q8_API int b200q8_dequantize_q4(void* out, int out_dtype, const uint8_t* q4,
 
 /* out[M, N] = inp[M, K] . w[N, K]^T + bias[N]; bias may be NULL.  inp and out are fp32 or fp16; any M.
  * Weights are used as they are, q * s with all its bits, and sums are fp32, whatever the types.  What is rounded
- * before them: at up to 8 tokens (16 for some shapes; fp32 inputs at any number) an input, by at most
- * 2^-22 of the largest |inp| of its 128 consecutive ones, or 2^-123; above, with fp16 inputs, a
- * scale below 2^-29 of its row's largest.  Scales' magnitudes are to be below 2^90.
+ * before them: with fp32 inputs, and fp16 at one or two tokens, an input, by at most 2^-22 of the
+ * largest |inp| of its 128 consecutive ones, or 2^-123; with fp16 inputs and more than 8 tokens, a scale
+ * below 2^-29 of its row's largest.  Scales' magnitudes are to be below 2^90.
  * An infinity or NaN in inp reaches its own row of out only, as the formula has it.
  * K a multiple of 32 with inp and q4 16-byte and scales 4-byte aligned is fast; the rest is correct.
- * fp16 calls of more than 8 tokens share a scratch per stream, allocated (cudaMalloc) with the first such
+ * fp16 calls of more than 8 tokens may share a scratch per stream, allocated (cudaMalloc) with the first such
  * call and kept.  Captured into a graph they get scratch of the graph's own, also where
  * it is the stream's first call: graphs may be replayed on any streams, beside each other. */
 B200Q8_API int b200q8_linear_q4(void* out, int out_dtype, const void* inp, int in_dtype, const uint8_t* q4,

@@ -248,3 +248,27 @@ def test_linear_repeats_bit_for_bit(cuda):
         first = _run_linear(cuda, x, q, s, 128, "float16", "float32")
         for _ in range(3):
             assert np.array_equal(first, _run_linear(cuda, x, q, s, 128, "float16", "float32"))
+
+
+@pytest.mark.parametrize("M", [1, 5, 12, 40, 130, 300])
+@pytest.mark.parametrize("K,group", [(896, 32), (3584, 128), (18944, 64)])
+@pytest.mark.parametrize("xdt", ["float16", "float32"])
+def test_fp32_outputs_are_fp32_sums(cuda, M, K, group, xdt):
+    """However many tokens and however long the sums.  A sum of at most K / 32 group sums, each rounded to 2^-24
+    of itself, whose errors are as good as independent: about sqrt(592) * 2^-24 * (a partial sum's mean size,
+    half) < 7.3e-7 of the result's deviation; the inputs' own rounding adds 2^-22 of a chunk's largest, 4 deviations
+    at most: 4 * 2^-22 / sqrt(12) < 2.8e-7."""
+    import torch
+
+    import vvllm_b200 as v
+
+    N = 640
+    g = torch.Generator(device=cuda).manual_seed(K + M)
+    q4 = torch.randint(0, 256, (N, K // 2), dtype=torch.uint8, device=cuda, generator=g)
+    sc = (0.001 + 0.01 * torch.rand((N, K // group), device=cuda, generator=g)).bfloat16()
+    x = torch.randn((M, K), device=cuda, generator=g).to(getattr(torch, xdt))
+    w, out = torch.empty((N, K), device=cuda), torch.empty((M, N), device=cuda)
+    v.dequantize_q4(w, q4, sc, group)
+    v.linear_q4(out, x, q4, sc, group)
+    want = x.double() @ w.double().T
+    assert float((out.double() - want).norm() / want.norm()) <= 1.1e-6

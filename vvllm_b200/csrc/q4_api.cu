@@ -95,15 +95,15 @@ int linear_q4(const char* what, void* out, int out_dtype, const void* inp, int i
     a.group = group;
     a.in_dtype = in_dtype;
     a.out_dtype = out_dtype;
-    // Up to 8 tokens the streaming kernel reads the weights once; above, once for every 8, where the GEMM
-    // (fp16 tokens) reads them once at a rate bound by its dequantization.  Measured on B200, streaming vs GEMM:
-    // 37888 x 3584 at 8 tokens 22 vs 37 us, at 9 36 vs 38, at 16 45 vs 38; 3584 x 18944 at 8 25 vs 28, at 16 49 vs 28.
-    // For 9 to 16 tokens and few weights with a long K, of which the GEMM makes few tiles, two passes still
-    // win: 3584 x 3584 at 16 19 vs 19, 896 x 4864 19 vs 24, 512 x 18944 28 vs 32; not 4864 x 896, 14 vs 10.
+    // Up to 16 fp16 tokens (8 in fp32) the streaming kernel reads the weights once; above, once for every so many,
+    // where the GEMM (fp16 tokens) reads them once at a rate bound by its dequantization.  Measured on B200,
+    // streaming vs GEMM: 37888 x 3584 at 16 tokens 24 vs 38 us, at 17 38 vs 38, at 32 48 vs 38; 896 x 4864 at 16 8 vs
+    // 24.  Tokens that need clusters of eight are slower: 3584 x 18944 at 9 24 vs 28, at 16 38 vs 28;
+    // 8192 x 28672 at 8 38 vs 64, at 9 72 vs 64.
     // fp32 outputs take the GEMM only with short sums: the tensor core's accumulator drops what falls below its 24
     // bits instead of rounding it, 1.8e-8 of the sum per 16 products (512 tokens, K = 18944: 2.2e-5 off, where
     // fp32 sums in another order are 2e-6 off and the streaming kernel's 3e-7); half an fp16 step is 2^-12.
-    const bool gemm = (M > 16 || (M > 8 && (N * K > ((size_t)1 << 24) || K < 2048))) && (out_dtype == B200Q8_F16 || K <= 512);
+    const bool gemm = (M > 16 || (M > 8 && M * K > 200 * 1024)) && (out_dtype == B200Q8_F16 || K <= 512);
     cudaError_t e;
     if (gemm && q4_gemm_tc_supports(a)) {
         size_t ws = 0, counters = 0, act = 0;

@@ -81,10 +81,14 @@ cudaError_t launch_generic(const Q4Args& a, cudaStream_t stream)
 
 
 // ----------------------------------------------------------------------------------------------
-// Streaming kernel: K % 32 == 0, aligned pointers, up to 8 tokens.
+// Streaming kernel: K % 32 == 0, aligned pointers, up to 16 tokens (8 in fp32).
 //
-// Exact integer products on the tensor cores.  A token's 128 consecutive elements ("chunk") become
-// integers X = rint(x * 2^(22 - e)), 2^e above the chunk's largest |x|, and X three signed bytes
+// Three to sixteen fp16 tokens: the codes become the integers q in fp16 (nine operations per eight), and
+// mma.sync m16n8k16 multiplies them with the tokens as they are; products are exact, the tensor core sums a
+// group's, and the group's sum times its scale is added to the row's in fp32.
+//
+// One or two tokens, and fp32 tokens: exact integer products.  A token's 128 consecutive elements ("chunk")
+// become integers X = rint(x * 2^(22 - e)), 2^e above the chunk's largest |x|, and X three signed bytes
 // X = 65536 X2 + 256 X1 + X0: three columns of the product.  The codes become bytes 16 q with three
 // integer operations per eight (one shift, two and-xor).  So mma.sync m16n8k32 (s8) sums 16 q * Xd
 // of a group exactly, and in fp32 every group's sum is multiplied by the group's scale and the
@@ -92,16 +96,17 @@ cudaError_t launch_generic(const Q4Args& a, cudaStream_t stream)
 // chunk's largest (fp16 tokens are exact down to 2^-11 of it), and the fp32 sums, once a group.  A chunk that
 // holds an infinity or NaN is summed directly instead.  Chunks below 2^-100 count as below 2^-100.
 //
-// Why not fp16 operands: unpacking to fp16 takes 18 operations per 16 x 32 weights and two products,
-// to bytes 6 and one; for one token and 37888 x 3584 the fp16 form of this kernel ran at 17.9 us,
-// bound by instruction issue, where this one takes 13.4.  Why not tcgen05: its operands would have to be
-// written back to shared or tensor memory as bytes, twice what was read; at 8 cycles a product, one
-// per three columns of 16 x 32 weights, mma.sync is within what HBM allows (about 44 cycles) to 13 tokens.
+// Why both: bytes take a third of the unpacking and half the products, which decides for one token (37888 x 3584:
+// in fp16 17.9 us, here 13.4); but each token is three columns and has to be taken apart in every CTA, which
+// decides from three on (8 tokens: in bytes 22.5 us, in fp16 17.1; 3584 x 3584 9.3 and 5.7).  Why not
+// tcgen05: its operands would have to be written back to shared or tensor memory, twice to four times
+// what was read; at 8 cycles a product, mma.sync is within what HBM allows (about 44 cycles for 16 x 32
+// weights) to 16 tokens.
 //
 // Bound by HBM (half a byte a weight) for one and two tokens once there are megabytes to stream: 152064 x 3584
-// at 46 us, 6.1 TB/s; 37888 x 3584 at 13.4 us, of which 3 are start and tokens.  At three to eight tokens by
-// instruction issue and its dependences, 33 instructions a 16 x 32 block: 152064 x 3584 73 us, 37888 x 3584 22 us,
-// at eight; with long K also by the tokens' way into shared memory: 3584 x 18944 12 us at one, 25 at eight.
+// at 46 us, 6.1 TB/s; 37888 x 3584 at 13.4 us, of which 3 are start and tokens.  With more, by instruction issue
+// and its dependences: 8 tokens, 152064 x 3584 64 us, 37888 x 3584 17; 16 tokens 93 and 24.5; with long K also by
+// the tokens' way into shared memory: 3584 x 18944 12 us at one, 17.5 at eight.
 //
 // Work: a tile is 16 rows; an item is a tile's next 256 or 512 of K.  `wk` warps share a tile (item ch
 // goes to warp ch mod wk) and add their sums through shared memory in warp order; a CTA of 8 or 16
@@ -123,7 +128,8 @@ constexpr int kMaxWarps = 16;
 constexpr int kBoxK = 256;  // K of one copied box: 128 bytes of each of 16 rows
 constexpr int kBoxBytes = 16 * 128;
 constexpr int kMaxStages = 4;
-constexpr int kMaxTokens = 8;
+constexpr int kMaxTokens = 16;      // of one launch: fp16 in halves,
+constexpr int kMaxDigitTokens = 8;  // in digits
 constexpr uint64_t kWaitNs = 4000000000ull;  // far above any legitimate wait
 
 struct StreamParams {
@@ -189,6 +195,38 @@ __device__ __forceinline__ void mma16832(int (&d)[4], int start, uint32_t a0, ui
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The eight codes of a word as the integers q in fp16: elements (0, 4), (1, 5), (2, 6), (3, 7).  A code in the low
+// bits of 1024.0 is 1024 + code, one four bits up 1024 + 16 code; one packed fma leaves q.
+__device__ __forceinline__ void unpack8_halves(uint32_t w, uint32_t (&h)[4])
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t v = i < 2 ? w : w >> 8;
+        if (i & 1) {
+            asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(h[i]) : "r"(v), "r"(0x00F000F0u), "r"(0x64006400u));
+            asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(h[i]) : "r"(0x2C002C00u), "r"(0xD480D480u));  // / 16 - 72
+        } else {
+            asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(h[i]) : "r"(v), "r"(0x000F000Fu), "r"(0x64006400u));
+            asm("add.rn.f16x2 %0, %0, %1;" : "+r"(h[i]) : "r"(0xE408E408u));  // - 1032
+        }
+    }
+}
+
+// d += A (16 x 16, fp16, rows) * B (16 x 8, fp16, columns), or with kFirst d = A * B; fp32 sums
+template <bool kFirst>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1)
+{
+    if constexpr (kFirst)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 // The sums start at the bit pattern of 1.5 * 2^23: read as a float they are that plus the sum, exact
 // while |sum| < 2^22 (a group's is at most 128 * 128 * 128 = 2^21).
 constexpr int kMagicBits = 0x4B400000;
@@ -200,9 +238,9 @@ __device__ __forceinline__ float2 tile_value(const int (&d)[4], int i)
     return __fadd2_rn(make_float2(__int_as_float(d[2 * i]), __int_as_float(d[2 * i + 1])), make_float2(-kMagic, -kMagic));
 }
 
-// Shared memory distance of two columns of `blocks` 32-blocks of bytes, two blocks to 64 bytes: an odd
-// number of those, so that neighbouring columns' loads fall into different banks.
-__host__ __device__ constexpr size_t column_stride(int blocks) { return (size_t)((blocks / 2) | 1) * 64; }
+// Shared memory distance of two columns of `blocks` 32-blocks, of bytes (two blocks to 64 bytes) or fp16 (one): an
+// odd number of those, so that neighbouring columns' loads fall into different banks.
+__host__ __device__ constexpr size_t column_stride(int blocks, bool halves) { return (size_t)((halves ? blocks : blocks / 2) | 1) * 64; }
 
 // Columns of the product.  Up to two tokens: one 8-column tile, token m's byte d (X0, X1, X2) in column
 // 3 m + d.  Up to eight: three tiles, token m in column m of tile d.
@@ -227,7 +265,7 @@ __device__ __forceinline__ bool stage_tokens(unsigned char* xs, float* weight, u
     constexpr int U = 5;  // chunks whose loads are in flight
     constexpr int kRaw = kF16 ? 4 : 8;
     const int K = (int)p.a.K, chunks = blocks / 4;
-    const size_t cs = column_stride(blocks);
+    const size_t cs = column_stride(blocks, false);
     const int u = threadIdx.x & 15;  // word of the chunk
     const int half = threadIdx.x >> 4, halves = blockDim.x >> 4;
     const int o = u & (4 * W - 1), ub = u / (4 * W) * W + (o & (W - 1));  // its block in the chunk
@@ -321,6 +359,48 @@ __device__ __forceinline__ bool stage_tokens(unsigned char* xs, float* weight, u
     return any;
 }
 
+// fp16 tokens as they are: [column m][block][quarter t] of eight, elements 0 4 1 5 2 6 3 7 of the word that lane t
+// multiplies with its word of the block (the words in the order above).  Zero behind K.
+template <class Asked, class Arrived>
+__device__ __forceinline__ void stage_halves(unsigned char* xs, const StreamParams& p, int W, int block0, int blocks, Asked asked,
+                                             Arrived arrived)
+{
+    constexpr int U = 8;  // chunks whose loads are in flight
+    const int K = (int)p.a.K, chunks = blocks / 4;
+    const size_t cs = column_stride(blocks, true);
+    const int u = threadIdx.x & 15, half = threadIdx.x >> 4, halves = blockDim.x >> 4;
+    const int o = u & (4 * W - 1), ub = u / (4 * W) * W + (o & (W - 1));
+    unsigned char* const dst0 = xs + ub * 64 + (o / W) * 16;
+    bool first = true;
+    for (int m = 0, c0 = 0; m < p.M;) {
+        uint4 raw[U];
+        int lm = m, lc = c0;
+#pragma unroll
+        for (int q = 0; q < U; q++) {
+            const int k = block0 * 32 + (lc + half) * 128 + u * 8;
+            raw[q] = make_uint4(0, 0, 0, 0);
+            if (lm < p.M && lc + half < chunks && k < K)
+                raw[q] = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.a.x) + (size_t)lm * K + k);
+            lc += halves;
+            if (lc >= chunks) lc = 0, lm++;
+        }
+        if (first) asked();
+#pragma unroll
+        for (int q = 0; q < U; q++) {
+            if (m >= p.M) break;  // uniform in the CTA
+            const uint4 r = raw[q];
+            const uint4 v = make_uint4(__byte_perm(r.x, r.z, 0x5410), __byte_perm(r.x, r.z, 0x7632),
+                                       __byte_perm(r.y, r.w, 0x5410), __byte_perm(r.y, r.w, 0x7632));
+            if (first) arrived();
+            first = false;
+            const int c = c0 + half;
+            if (c < chunks) *reinterpret_cast<uint4*>(dst0 + c * 256 + m * cs) = v;
+            c0 += halves;
+            if (c0 >= chunks) c0 = 0, m++;
+        }
+    }
+}
+
 // A warp adds to sums[r], r < 16, token m's products with rows tile * 16 + r over 128-chunk c, as the formula
 // reads: what infinities and NaN need.
 __device__ __noinline__ void direct_chunk(const Q4Args& a, float* sums, int tile, int m, int c)
@@ -350,28 +430,33 @@ __device__ __noinline__ void direct_chunk(const Q4Args& a, float* sums, int tile
     __syncwarp();
 }
 
-template <int NT, int IB>
+template <int NT, int IB, bool kHalves>
 struct StreamCfg {
     static constexpr int kItemBytes = IB * kBoxBytes;
     static constexpr int kChunks = IB * kBoxK / 128;  // 128-chunks of an item
-    static constexpr int kCols = 8;                   // columns kept in `weight`: NT == 1 the tile's, else the tokens
-    static constexpr int kSums = NT == 1 ? 2 * 16 : 8 * 16;  // a tile's outputs: [token][row]
+    static constexpr int kCols = kHalves ? 0 : 8;     // columns kept in `weight`: NT == 1 the tile's, else the tokens
+    static constexpr int kChunkBytes = kHalves ? 256 : 128;  // of a column
+    static constexpr int kOut = kHalves ? NT : 1;            // eights of tokens in a lane's sums
+    static constexpr int kSums = (kHalves ? 8 * NT : NT == 1 ? 2 : 8) * 16;  // a tile's outputs: [token][row]
     // Two buffers of sums, read while the next tile's are written, where warps or CTAs share a tile.
     static constexpr int red_bufs(int wk, int cluster) { return wk == 1 && cluster == 1 ? 1 : 2; }
     static size_t smem(int warps, int stages, int M, int per, int cluster, int wk)
     {
         const int chunks = per * kChunks;
-        return 1024 + (size_t)warps * stages * kItemBytes + warps * kMaxStages * 8 + 3 * M * column_stride(chunks * 4) +
-               (size_t)chunks * kCols * 4 + (size_t)red_bufs(wk, cluster) * warps * kSums * 4 +
-               (cluster > 1 ? (size_t)2 * cluster * (warps / wk) * kSums * 4 : 0) + (size_t)M * chunks;
+        return 1024 + (size_t)warps * stages * kItemBytes + warps * kMaxStages * 8 +
+               (kHalves ? 1 : 3) * M * column_stride(chunks * 4, kHalves) + (size_t)chunks * kCols * 4 +
+               (size_t)red_bufs(wk, cluster) * warps * kSums * 4 +
+               (cluster > 1 ? (size_t)2 * cluster * (warps / wk) * kSums * 4 : 0) + (kHalves ? 0 : (size_t)M * chunks);
     }
 };
 
-template <int NT, int G, int IB>
+// kHalves false: the tokens' digits in NT = 1 (up to two tokens) or 3 (up to eight) tiles of eight columns; true: up to
+// 8 NT fp16 tokens as they are.
+template <int NT, int G, int IB, bool kHalves>
 __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     q4_stream_kernel(const __grid_constant__ CUtensorMap tmW, const StreamParams p)
 {
-    using C = StreamCfg<NT, IB>;
+    using C = StreamCfg<NT, IB, kHalves>;
     constexpr int kItemBytes = C::kItemBytes;
     constexpr int W = G / 32;   // words a lane holds of a group; 32-blocks of a group
     constexpr int GC = 128 / G;  // groups of a chunk
@@ -387,8 +472,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (size_t)warps * p.stages * kItemBytes);
     unsigned char* xs = reinterpret_cast<unsigned char*>(bars + warps * kMaxStages);
     const int xchunks = p.per * C::kChunks;
-    const size_t cs = column_stride(xchunks * 4);
-    float* weight = reinterpret_cast<float*>(xs + 3 * p.M * cs);
+    const size_t cs = column_stride(xchunks * 4, kHalves);
+    float* weight = reinterpret_cast<float*>(xs + (kHalves ? 1 : 3) * p.M * cs);
     float* red = weight + xchunks * C::kCols;         // [buffer][warp][tile's outputs]
     float* cbuf = red + C::red_bufs(p.wk, csize) * warps * C::kSums;  // [2][rank][group][tile's outputs] of a cluster's CTAs (in rank 0)
     unsigned char* direct = reinterpret_cast<unsigned char*>(cbuf + (csize > 1 ? 2 * csize * (warps >> p.wk_log2) * C::kSums : 0));
@@ -505,17 +590,25 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
         if (lane == 0)
             for (; inflight < p.stages && itile < p.tiles; inflight++, advance()) load_item(inflight);
     };
-    const bool some = p.a.in_dtype == kF16
-                          ? stage_tokens<NT, true>(xs, weight, direct, p, W, ch0 * C::kChunks * 4, xchunks * 4, asked, arrived)
-                          : stage_tokens<NT, false>(xs, weight, direct, p, W, ch0 * C::kChunks * 4, xchunks * 4, asked, arrived);
-    const bool any_direct = __syncthreads_or(some);
+    bool any_direct = false;
+    if constexpr (kHalves) {
+        stage_halves(xs, p, W, ch0 * C::kChunks * 4, xchunks * 4, asked, arrived);
+        __syncthreads();
+    } else {
+        const int block0 = ch0 * C::kChunks * 4, blocks = xchunks * 4;
+        any_direct = __syncthreads_or(p.a.in_dtype == kF16
+                                          ? stage_tokens<NT, true>(xs, weight, direct, p, W, block0, blocks, asked, arrived)
+                                          : stage_tokens<NT, false>(xs, weight, direct, p, W, block0, blocks, asked, arrived));
+    }
     if (csize > 1) cluster.sync();  // every rank runs before rank 0's memory is stored to
 
     uint32_t xoff[NT];  // this lane's column of each 8-column tile (lanes behind the last column repeat it)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
         xoff[nt] = tc::smem_u32(xs) + t * 16 +
-                   (uint32_t)((NT == 1 ? min(g, 3 * p.M - 1) : nt * p.M + min(g, p.M - 1)) * cs);
+                   (uint32_t)((kHalves   ? min(nt * 8 + g, p.M - 1)
+                               : NT == 1 ? min(g, 3 * p.M - 1)
+                                         : nt * p.M + min(g, p.M - 1)) * cs);
     // The lane's words of group 0 of a box: 16-byte piece ((t * W) / 4) ^ row of its row; another group is an
     // XOR away.
     const uint32_t wlane = row * 128 + ((((t * W) >> 2) ^ row) << 4) + ((t * W) & 3) * 4;
@@ -530,7 +623,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
         if (tile >= p.tiles && csize == 1) break;  // a cluster's groups end together, for its barriers
         if (lane == 0 && kw == 0 && tile + tstep < p.tiles) prefetch_scales(tile + tstep);
         // Of rows row and row + 8: columns 2t and 2t + 1, which are tokens where three tiles hold their bytes.
-        float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        float2 acc[C::kOut][2];
+#pragma unroll
+        for (int o = 0; o < C::kOut; o++) acc[o][0] = acc[o][1] = make_float2(0.0f, 0.0f);
         for (int ch = ch0 + kw; ch < ch1 && tile < p.tiles; ch += wk) {
             if (ok) {
                 ok = __all_sync(0xffffffffu, tc::mbar_wait(bar0 + 8 * stage, phase, &zero, kWaitNs));
@@ -538,7 +633,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
             }
             uint32_t wrow = ring + stage * kItemBytes + wlane;
             fence(wrow);
-            uint32_t xitem = (uint32_t)(ch - ch0) * (C::kChunks * 128);
+            uint32_t xitem = (uint32_t)(ch - ch0) * (C::kChunks * C::kChunkBytes);
             const float* wchunk = weight + (ch - ch0) * C::kChunks * C::kCols + 2 * t;
             // Chunks behind K need no care: their codes and tokens are zeros, and so are their scales.
             Scales sc_after = sc;
@@ -547,57 +642,93 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
             for (int box = 0; box < IB; box++) {
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    uint32_t x[NT][2][4];
+                    if constexpr (kHalves) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        lds<4>(xoff[nt] + xitem + c * 128, x[nt][0]);
-                        lds<4>(xoff[nt] + xitem + c * 128 + 64, x[nt][1]);
-                    }
-                    float2 sum[2];
+                        for (int gi = 0; gi < GC; gi++) {
+                            uint32_t w0[W], w1[W];
+                            lds<W>(wrow ^ (c * 64 + gi * W * 16), w0);
+                            lds<W>((wrow ^ (c * 64 + gi * W * 16)) + 1024, w1);
+                            float d[NT][4];
 #pragma unroll
-                    for (int gi = 0; gi < GC; gi++) {
-                        uint32_t w0[W], w1[W];
-                        lds<W>(wrow ^ (c * 64 + gi * W * 16), w0);
-                        lds<W>((wrow ^ (c * 64 + gi * W * 16)) + 1024, w1);
-                        int d[NT][4];
+                            for (int b = 0; b < W; b++) {
+                                uint32_t x[NT][4], h0[4], h1[4];
 #pragma unroll
-                        for (int b = 0; b < W; b++) {
-                            const int blk = gi * W + b;
-                            uint32_t a0, a1, a2, a3;
-                            unpack8(w0[b], a0, a2);
-                            unpack8(w1[b], a1, a3);
+                                for (int nt = 0; nt < NT; nt++) lds<4>(xoff[nt] + xitem + c * 256 + (gi * W + b) * 64, x[nt]);
+                                unpack8_halves(w0[b], h0);
+                                unpack8_halves(w1[b], h1);
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++) {
-                                const uint32_t b0 = x[nt][blk >> 1][2 * (blk & 1)], b1 = x[nt][blk >> 1][2 * (blk & 1) + 1];
-                                if (b == 0)
-                                    mma16832<true>(d[nt], kMagicBits, a0, a1, a2, a3, b0, b1);
-                                else
-                                    mma16832<false>(d[nt], 0, a0, a1, a2, a3, b0, b1);
+                                for (int nt = 0; nt < NT; nt++) {
+                                    if (b == 0)
+                                        mma16816<true>(d[nt], h0[0], h1[0], h0[1], h1[1], x[nt][0], x[nt][1]);
+                                    else
+                                        mma16816<false>(d[nt], h0[0], h1[0], h0[1], h1[1], x[nt][0], x[nt][1]);
+                                    mma16816<false>(d[nt], h0[2], h1[2], h0[3], h1[3], x[nt][2], x[nt][3]);
+                                }
+                            }
+                            const int si = c * GC + gi;
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                const uint32_t word = i == 0 ? sc.a[box][si / 2] : sc.b[box][si / 2];
+                                const float r = __uint_as_float(si & 1 ? word & 0xFFFF0000u : word << 16);
+#pragma unroll
+                                for (int nt = 0; nt < NT; nt++)
+                                    acc[nt][i] = __ffma2_rn(make_float2(d[nt][2 * i], d[nt][2 * i + 1]), make_float2(r, r), acc[nt][i]);
                             }
                         }
-                        const int si = c * GC + gi;
+                    } else {
+                        uint32_t x[NT][2][4];
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const uint32_t word = i == 0 ? sc.a[box][si / 2] : sc.b[box][si / 2];
-                            const float r = __uint_as_float(si & 1 ? word & 0xFFFF0000u : word << 16);
-                            float2 f = tile_value(d[0], i);
-                            if constexpr (NT == 3)  // X0 + 256 X1 + 65536 X2
-                                f = __ffma2_rn(__ffma2_rn(tile_value(d[2], i), make_float2(256.0f, 256.0f), tile_value(d[1], i)),
-                                               make_float2(256.0f, 256.0f), f);
-                            sum[i] = gi == 0 ? __fmul2_rn(f, make_float2(r, r)) : __ffma2_rn(f, make_float2(r, r), sum[i]);
+                        for (int nt = 0; nt < NT; nt++) {
+                            lds<4>(xoff[nt] + xitem + c * 128, x[nt][0]);
+                            lds<4>(xoff[nt] + xitem + c * 128 + 64, x[nt][1]);
                         }
+                        float2 sum[2];
+#pragma unroll
+                        for (int gi = 0; gi < GC; gi++) {
+                            uint32_t w0[W], w1[W];
+                            lds<W>(wrow ^ (c * 64 + gi * W * 16), w0);
+                            lds<W>((wrow ^ (c * 64 + gi * W * 16)) + 1024, w1);
+                            int d[NT][4];
+#pragma unroll
+                            for (int b = 0; b < W; b++) {
+                                const int blk = gi * W + b;
+                                uint32_t a0, a1, a2, a3;
+                                unpack8(w0[b], a0, a2);
+                                unpack8(w1[b], a1, a3);
+#pragma unroll
+                                for (int nt = 0; nt < NT; nt++) {
+                                    const uint32_t b0 = x[nt][blk >> 1][2 * (blk & 1)], b1 = x[nt][blk >> 1][2 * (blk & 1) + 1];
+                                    if (b == 0)
+                                        mma16832<true>(d[nt], kMagicBits, a0, a1, a2, a3, b0, b1);
+                                    else
+                                        mma16832<false>(d[nt], 0, a0, a1, a2, a3, b0, b1);
+                                }
+                            }
+                            const int si = c * GC + gi;
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                const uint32_t word = i == 0 ? sc.a[box][si / 2] : sc.b[box][si / 2];
+                                const float r = __uint_as_float(si & 1 ? word & 0xFFFF0000u : word << 16);
+                                float2 f = tile_value(d[0], i);
+                                if constexpr (NT == 3)  // X0 + 256 X1 + 65536 X2
+                                    f = __ffma2_rn(__ffma2_rn(tile_value(d[2], i), make_float2(256.0f, 256.0f), tile_value(d[1], i)),
+                                                   make_float2(256.0f, 256.0f), f);
+                                sum[i] = gi == 0 ? __fmul2_rn(f, make_float2(r, r)) : __ffma2_rn(f, make_float2(r, r), sum[i]);
+                            }
+                        }
+                        const float2 wt = *reinterpret_cast<const float2*>(wchunk + c * C::kCols);
+                        acc[0][0] = __ffma2_rn(sum[0], wt, acc[0][0]);
+                        acc[0][1] = __ffma2_rn(sum[1], wt, acc[0][1]);
                     }
-                    const float2 wt = *reinterpret_cast<const float2*>(wchunk + c * C::kCols);
-                    acc[0] = __ffma2_rn(sum[0], wt, acc[0]);
-                    acc[1] = __ffma2_rn(sum[1], wt, acc[1]);
                 }
                 wrow += kBoxBytes;
-                xitem += 256;
+                xitem += 2 * C::kChunkBytes;
                 wchunk += 2 * C::kCols;
             }
             sc = IB == 1 ? sc_next : sc_after;
             sc_next = sc_after;
-            fence(acc[0].x), fence(acc[0].y), fence(acc[1].x), fence(acc[1].y);
+#pragma unroll
+            for (int o = 0; o < C::kOut; o++) fence(acc[o][0].x), fence(acc[o][0].y), fence(acc[o][1].x), fence(acc[o][1].y);
             __syncwarp();  // the stage is read
             if (ok) {  // else the ring stays as it is, for the end
                 if (lane == 0) {
@@ -614,17 +745,21 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
                 }
             }
         }
-        // ---- v[i] of rows row (i < 2) and row + 8, tokens mt and mt + 1 (NT == 1: mt only)
-        float v[4] = {acc[0].x, acc[0].y, acc[1].x, acc[1].y};
-        const int mt = NT == 1 ? t >> 1 : 2 * t;
-        if constexpr (NT == 1) {  // columns 0 1 | 2, 3 | 4 5 of lanes t = 0, 1, 2: a token's three bytes
-            const float a = __shfl_down_sync(0xffffffffu, v[0], 1), b = __shfl_down_sync(0xffffffffu, v[2], 1);
-            const float c = __shfl_up_sync(0xffffffffu, v[1], 1), d = __shfl_up_sync(0xffffffffu, v[3], 1);
-            v[0] = t == 0 ? v[0] + v[1] + a : c + v[0] + v[1];
-            v[2] = t == 0 ? v[2] + v[3] + b : d + v[2] + v[3];
+        // ---- v[o][i] of rows row (i < 2) and row + 8, tokens 8 o + mt and, but with digits in one tile, + 1
+        float v[C::kOut][4];
+#pragma unroll
+        for (int o = 0; o < C::kOut; o++)
+            v[o][0] = acc[o][0].x, v[o][1] = acc[o][0].y, v[o][2] = acc[o][1].x, v[o][3] = acc[o][1].y;
+        constexpr bool kOneTile = !kHalves && NT == 1;
+        const int mt = kOneTile ? t >> 1 : 2 * t;
+        if constexpr (kOneTile) {  // columns 0 1 | 2, 3 | 4 5 of lanes t = 0, 1, 2: a token's three bytes
+            const float a = __shfl_down_sync(0xffffffffu, v[0][0], 1), b = __shfl_down_sync(0xffffffffu, v[0][2], 1);
+            const float c = __shfl_up_sync(0xffffffffu, v[0][1], 1), d = __shfl_up_sync(0xffffffffu, v[0][3], 1);
+            v[0][0] = t == 0 ? v[0][0] + v[0][1] + a : c + v[0][0] + v[0][1];
+            v[0][2] = t == 0 ? v[0][2] + v[0][3] + b : d + v[0][2] + v[0][3];
         }
-        auto mine = [&](int i) {  // whether v[i] is an output's sum
-            return NT == 1 ? (t & 1) == 0 && (i & 1) == 0 && mt < p.M : mt + (i & 1) < p.M;
+        auto mine = [&](int o, int i) {  // whether v[o][i] is an output's sum
+            return kOneTile ? (t & 1) == 0 && (i & 1) == 0 && mt < p.M : 8 * o + mt + (i & 1) < p.M;
         };
         auto put = [&](int m, int r, float y) {
             const long long n = (long long)tile * 16 + r;
@@ -639,16 +774,20 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
         };
         if (wk == 1 && csize == 1 && !any_direct) {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (mine(i)) put(mt + (i & 1), row + 8 * (i >> 1), v[i]);
+            for (int o = 0; o < C::kOut; o++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (mine(o, i)) put(8 * o + mt + (i & 1), row + 8 * (i >> 1), v[o][i]);
             continue;
         }
         // ---- the tile's sums: warps in order, then cluster ranks in order
         float* rbuf = red + parity * warps * C::kSums;
         float* wsum = rbuf + warp * C::kSums;  // [token][row]
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (mine(i)) wsum[(mt + (i & 1)) * 16 + row + 8 * (i >> 1)] = v[i];
+        for (int o = 0; o < C::kOut; o++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (mine(o, i)) wsum[(8 * o + mt + (i & 1)) * 16 + row + 8 * (i >> 1)] = v[o][i];
         if (any_direct && tile < p.tiles) {  // rare: infinities or NaN among this CTA's elements
             __syncwarp();
             for (int m = 0; m < p.M; m++)
@@ -708,13 +847,14 @@ constexpr size_t kSmemPerSM = 228 * 1024;
 
 struct StreamPlan {
     int tokens = 0;  // of one launch; 0: the kernel cannot take the shape
+    bool halves = false;
     int nt = 0, ib = 1, cluster = 1, nch = 0, per = 0, warps = 8, wk = 8, stages = 0;
 };
 
-template <int NT, int G, int IB>
+template <int NT, int G, int IB, bool kHalves>
 cudaError_t launch_stream(const StreamParams& p, const StreamPlan& s, int num_sms, size_t max_smem, cudaStream_t stream)
 {
-    using C = StreamCfg<NT, IB>;
+    using C = StreamCfg<NT, IB, kHalves>;
     CUtensorMap mw;
     TmapDesc w{};
     w.base = p.a.q4;
@@ -726,7 +866,7 @@ cudaError_t launch_stream(const StreamParams& p, const StreamPlan& s, int num_sm
     w.dtype = CU_TENSOR_MAP_DATA_TYPE_UINT8;
     w.swizzle = CU_TENSOR_MAP_SWIZZLE_128B;
     if (!tmap_2d(&mw, w)) return cudaErrorInvalidValue;
-    auto kern = q4_stream_kernel<NT, G, IB>;
+    auto kern = q4_stream_kernel<NT, G, IB, kHalves>;
     static thread_local bool configured[64] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -783,23 +923,33 @@ cudaError_t launch_stream(const StreamParams& p, const StreamPlan& s, int num_sm
     return e;
 }
 
+template <int NT, int G, bool kHalves>
+cudaError_t launch_stream_ib(const StreamParams& p, const StreamPlan& s, int num_sms, size_t max_smem, cudaStream_t stream)
+{
+    return s.ib == 1 ? launch_stream<NT, G, 1, kHalves>(p, s, num_sms, max_smem, stream)
+                     : launch_stream<NT, G, 2, kHalves>(p, s, num_sms, max_smem, stream);
+}
+
 template <int G>
 cudaError_t launch_stream_nt(const StreamParams& p, const StreamPlan& s, int num_sms, size_t max_smem, cudaStream_t stream)
 {
-    if (s.nt == 1)
-        return s.ib == 1 ? launch_stream<1, G, 1>(p, s, num_sms, max_smem, stream)
-                         : launch_stream<1, G, 2>(p, s, num_sms, max_smem, stream);
-    return s.ib == 1 ? launch_stream<3, G, 1>(p, s, num_sms, max_smem, stream)
-                     : launch_stream<3, G, 2>(p, s, num_sms, max_smem, stream);
+    if (s.halves)
+        return s.nt == 1 ? launch_stream_ib<1, G, true>(p, s, num_sms, max_smem, stream)
+                         : launch_stream_ib<2, G, true>(p, s, num_sms, max_smem, stream);
+    return s.nt == 1 ? launch_stream_ib<1, G, false>(p, s, num_sms, max_smem, stream)
+                     : launch_stream_ib<3, G, false>(p, s, num_sms, max_smem, stream);
 }
 
-size_t stream_smem(int nt, int ib, int warps, int stages, int M, int per, int cluster, int wk)
+size_t stream_smem(int nt, int ib, bool halves, int warps, int stages, int M, int per, int cluster, int wk)
 {
-    if (nt == 1)
-        return ib == 1 ? StreamCfg<1, 1>::smem(warps, stages, M, per, cluster, wk)
-                       : StreamCfg<1, 2>::smem(warps, stages, M, per, cluster, wk);
-    return ib == 1 ? StreamCfg<3, 1>::smem(warps, stages, M, per, cluster, wk)
-                   : StreamCfg<3, 2>::smem(warps, stages, M, per, cluster, wk);
+    auto of = [&](auto one, auto two) {
+        return ib == 1 ? decltype(one)::smem(warps, stages, M, per, cluster, wk) : decltype(two)::smem(warps, stages, M, per, cluster, wk);
+    };
+    if (halves)
+        return nt == 1 ? of(StreamCfg<1, 1, true>(), StreamCfg<1, 2, true>())
+                       : of(StreamCfg<2, 1, true>(), StreamCfg<2, 2, true>());
+    return nt == 1 ? of(StreamCfg<1, 1, false>(), StreamCfg<1, 2, false>())
+                   : of(StreamCfg<3, 1, false>(), StreamCfg<3, 2, false>());
 }
 
 constexpr int kMaxCluster = 8;
@@ -808,24 +958,28 @@ constexpr int kMaxCluster = 8;
 // box's products: 37888 x 3584, one token, 14.9 us with one box, 13.4 with two), two items in flight a warp
 // (three: 14.4 us, the copies' queue then holds up the warps); sixteen warps an SM, in two CTAs where the
 // tokens leave room, else in one, else in clusters of 2, 4, 8; eight only where that does not fit either
-// (8 tokens, 4096 x 14336: 17 us in clusters of four, with eight warps in clusters of two 26).
+// (8 tokens in bytes, 4096 x 14336: 17 us in clusters of four, with eight warps in clusters of two 26).
 // One or two tokens take a cluster only where one CTA cannot hold them.  With more, putting them into shared memory
 // is what a CTA of few tiles spends its time on, so a long K is split over as many SMs as the tiles
-// leave free (8 tokens, 896 x 4864: 9.2 us on clusters of two, 12 without).
+// leave free (8 tokens in bytes, 896 x 4864: 9.6 us on clusters of two, 12 without), and over more where
+// that leaves warps less to do (9 tokens, 14336 x 8192: 32 us in clusters of two, in single CTAs 48).
 StreamPlan plan_stream(const Q4Args& a, size_t M, int num_sms, size_t max_smem)
 {
     const long long tiles = (long long)((a.N + 15) / 16);
-    for (int m = (int)std::min<size_t>(M, kMaxTokens); m >= 1; m--) {
-        const int nt = m <= 2 ? 1 : 3;
+    const bool f16 = a.in_dtype == kF16;
+    for (int m = (int)std::min<size_t>(M, f16 ? kMaxTokens : kMaxDigitTokens); m >= 1; m--) {
+        const bool halves = f16 && m > 2;
+        const int nt = m <= 2 ? 1 : !halves ? 3 : m <= 8 ? 1 : 2;
         int c0 = 1;
-        while (nt == 3 && c0 < kMaxCluster && 2 * c0 * tiles <= num_sms && a.K >= (size_t)4096 * c0) c0 *= 2;
-        for (int all = 1; all >= 0; all--)
-            for (int c = all ? c0 : 1; c <= kMaxCluster; c *= 2) {
-                StreamPlan found;
-                double best = 1e30;  // what a warp has to do, in boxes
-                for (int ib = all && a.K >= 2048 && (nt == 1 || c == 1) ? 2 : 1; ib >= 1; ib--) {
+        while (m > 2 && c0 < kMaxCluster && 2 * c0 * tiles <= num_sms && a.K >= (size_t)4096 * c0) c0 *= 2;
+        for (int all = 1; all >= 0; all--) {
+            StreamPlan found;
+            double best = 1e30;  // what a warp has to do, in boxes
+            for (int c = all ? c0 : 1; c <= kMaxCluster && !(m <= 2 && found.tokens); c *= 2)
+                for (int ib = all && a.K >= 2048 && (m <= 2 || c == 1) ? 2 : 1; ib >= 1; ib--) {
                     StreamPlan s;
                     s.tokens = m;
+                    s.halves = halves;
                     s.nt = nt;
                     s.ib = ib;
                     s.cluster = c;
@@ -840,11 +994,11 @@ StreamPlan plan_stream(const Q4Args& a, size_t M, int num_sms, size_t max_smem)
                         s.warps = warps;
                         for (s.wk = c > 1 ? 2 : 1; s.wk <= warps; s.wk *= 2) {
                             s.stages = ib == 2 ? 2 : 3;
-                            while (s.stages >= 2 && stream_smem(nt, ib, warps, s.stages, m, s.per, c, s.wk) > budget) s.stages--;
+                            while (s.stages >= 2 && stream_smem(nt, ib, halves, warps, s.stages, m, s.per, c, s.wk) > budget) s.stages--;
                             if (s.stages < 2) continue;
                             any = true;
                             const double join = c > 1 ? 2.7 : s.wk > 1 ? 1.5 : 0.75;
-                            const double cost = (double)((tiles * s.wk + slots - 1) / slots) * ((s.per + s.wk - 1) / s.wk * (ib + 0.33) + join);
+                            const double cost = (double)((tiles * s.wk + slots - 1) / slots) * ((s.per + s.wk - 1) / s.wk * (ib + 0.33) + join) * (c > c0 ? 1.15 : 1.0);
                             if (cost < best) best = cost, found = s;
                         }
                         return any;
@@ -854,8 +1008,8 @@ StreamPlan plan_stream(const Q4Args& a, size_t M, int num_sms, size_t max_smem)
                     else if (c > 1 || !fit(8, kSmemPerSM / 2 - 1024))
                         fit(16, max_smem);
                 }
-                if (found.tokens) return found;
-            }
+            if (found.tokens) return found;
+        }
     }
     return StreamPlan{};
 }
