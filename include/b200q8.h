@@ -277,9 +277,10 @@ B200Q8_API int b200q8_dequantize_q4(void* out, int out_dtype, const uint8_t* q4,
  * largest |inp| of its 128 consecutive ones, or 2^-123; with fp16 inputs and more than 8 tokens, a scale
  * below 2^-29 of its row's largest.  Scales' magnitudes are to be below 2^90.
  * An infinity or NaN in inp reaches its own row of out only, as the formula has it.
- * K a multiple of 32 with inp and q4 16-byte and scales 4-byte aligned is fast; the rest is correct.
- * fp16 calls of more than 8 tokens may share a scratch per stream, allocated (cudaMalloc) with the first such
- * call and kept.  Captured into a graph they get scratch of the graph's own, also where
+ * K a multiple of 32 with inp and q4 16-byte aligned is read as it lies; else larger calls first copy
+ * the weights and tokens into such rows, in scratch of their size.
+ * These and fp16 calls of more than 8 tokens share a scratch per stream, allocated (cudaMalloc) with the first
+ * such call, grown where a call needs more, and kept.  Captured into a graph they get scratch of the graph's own, also where
  * it is the stream's first call: graphs may be replayed on any streams, beside each other. */
 B200Q8_API int b200q8_linear_q4(void* out, int out_dtype, const void* inp, int in_dtype, const uint8_t* q4,
                                 const uint16_t* scales, int group, const float* bias, size_t M, size_t N, size_t K,

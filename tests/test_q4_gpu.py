@@ -272,3 +272,44 @@ def test_fp32_outputs_are_fp32_sums(cuda, M, K, group, xdt):
     v.linear_q4(out, x, q4, sc, group)
     want = x.double() @ w.double().T
     assert float((out.double() - want).norm() / want.norm()) <= 1.1e-6
+
+
+@pytest.mark.parametrize("odt", ["float16", "float32"])
+@pytest.mark.parametrize("xdt", ["float16", "float32"])
+@pytest.mark.parametrize("M,N,K", [(1, 77, 1001), (2, 130, 3583), (8, 33, 999), (9, 129, 801), (16, 300, 2047), (17, 65, 1030),
+                                   (40, 300, 775), (130, 200, 1250), (5, 50, 18943), (100, 300, 77)])
+def test_linear_rows_that_are_copied_first(cuda, M, N, K, xdt, odt):
+    """K no multiple of 32, large enough to be copied into padded rows (and one that is not)."""
+    _check_integers(cuda, M, N, K, 64, xdt, odt)
+
+
+@pytest.mark.parametrize("what", ["q4", "x"])
+@pytest.mark.parametrize("M,N,K", [(1, 100, 1024), (8, 70, 2048), (40, 300, 1024)])
+def test_linear_large_unaligned_pointers(cuda, what, M, N, K):
+    import torch
+
+    import vvllm_b200 as v
+
+    q, s, x, _, _ = _integer_case(M, N, K, 128, 5)
+    t = {"q4": torch.from_numpy(u.pack(q)).to(cuda), "x": torch.from_numpy(x).to(cuda).half()}
+    sc, want = _scales_t(s, cuda), u.linear(x, q, s, 128)
+    for off in (1, 2, 3, 7):
+        big = torch.zeros(t[what].numel() + off, dtype=t[what].dtype, device=cuda)
+        big[off:] = t[what].reshape(-1)
+        view, out = dict(t), torch.empty((M, N), device=cuda)
+        view[what] = big[off:].view(t[what].shape)
+        v.linear_q4(out, view["x"], view["q4"], sc, 128)
+        assert np.array_equal(out.cpu().numpy(), want.astype(np.float32)), off
+
+
+@pytest.mark.parametrize("M", [1, 12])
+def test_linear_bad_tokens_stay_in_their_row_when_copied(cuda, M):
+    N, K = 90, 1003
+    q, s, x, _, _ = _integer_case(M + 2, N, K, 64, 8)
+    x = x.copy()
+    x[0, 1002], x[-1, 3] = np.inf, np.nan
+    got = _run_linear(cuda, x, q, s, 64, "float16", "float32")
+    with np.errstate(invalid="ignore"):
+        y = u.linear(x, q, s, 64)
+    assert np.array_equal(got[1:-1], y[1:-1].astype(np.float32)) and np.isnan(got[-1]).all()
+    assert np.array_equal(np.isfinite(got[0]), np.isfinite(y[0]))

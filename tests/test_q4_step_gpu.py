@@ -217,6 +217,36 @@ def test_graphs_of_one_stream_run_beside_each_other_and_beside_its_calls(cuda):
         del graphs, g
 
 
+def test_copied_rows_in_graphs(cuda):
+    """Calls whose rows are copied first: from graphs of one stream side by side, beside calls there."""
+    import torch
+
+    import vvllm_b200 as v
+
+    st, others, jobs, graphs = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)], [], []
+    for i, M in enumerate((1, 40, 6)):
+        r = np.random.default_rng(i)
+        q, s = r.integers(-8, 8, (500, 1021)), 2.0 ** r.integers(-2, 1, (500, 16))
+        x = r.integers(-3, 4, (M, 1021)).astype(np.float64)
+        jobs.append((torch.from_numpy(x).to(cuda).half(), torch.from_numpy(u.pack(q)).to(cuda),
+                     torch.from_numpy(u.bf16_bits(s).view(np.int16)).to(cuda).view(torch.bfloat16),
+                     u.linear(x, q, s, 64).astype(np.float32), torch.empty((M, 500), device=cuda)))
+    torch.cuda.synchronize()
+    for x, q4, sc, _, out in jobs[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            v.linear_q4(out, x, q4, sc, 64, stream=st)
+        graphs.append(g)
+    for _ in range(20):
+        for g, o in zip(graphs, others):
+            with torch.cuda.stream(o):
+                g.replay()
+        v.linear_q4(jobs[2][4], *jobs[2][:3], 64, stream=st)
+    torch.cuda.synchronize()
+    for _, _, _, want, out in jobs:
+        assert np.array_equal(out.cpu().numpy(), want)
+
+
 def test_two_branches_of_one_capture(cuda):
     """Calls on two streams of one capture run beside each other in the graph."""
     import torch

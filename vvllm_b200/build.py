@@ -22,7 +22,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libb200q8.so")
 
 SOURCES = ["b200q8_api.cu", "q8_gemv.cu", "q8_quantize.cu", "q8_gemm_tc.cu", "q8_gemv_tc.cu", "gather.cu", "prologue.cu", "q8st.cu",
-           "q4_api.cu", "q4_quantize.cu", "q4_gemv.cu", "logits.cu"]
+           "q4_api.cu", "q4_pad.cu", "q4_quantize.cu", "q4_gemv.cu", "logits.cu"]
 HEADERS = ["common.cuh", "kernels.h", "tc_utils.cuh", "sk_common.cuh", "tmap.cuh", "prologue.cuh", "p2p.cuh",
            "q4_common.cuh"]
 

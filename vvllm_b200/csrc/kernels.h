@@ -172,7 +172,11 @@ struct Q4Args {
 };
 // Any shape and alignment.
 cudaError_t launch_q4_linear_generic(const Q4Args& a, cudaStream_t stream);
-// Streaming tensor-core kernel: K % 32 == 0, q4 and x 16-byte, scales 4-byte aligned.  Any M, in passes of
+// The kernels below take K % 32 == 0 with q4 and x 16-byte aligned.  Bytes of scratch (16-byte aligned) that it takes to
+// bring other calls there, and the copying, after which *a is such a call.
+size_t q4_pad_bytes(const Q4Args& a);
+cudaError_t launch_q4_pad(Q4Args* a, unsigned char* to, int num_sms, cudaStream_t stream);
+// Streaming tensor-core kernel: K % 32 == 0, q4 and x 16-byte aligned.  Any M, in passes of
 // up to 16 (fp16) or 8 (fp32) tokens.  cudaErrorNotSupported: alignment, or K beyond its shared memory.
 bool q4_stream_supports(const Q4Args& a);
 cudaError_t launch_q4_stream(const Q4Args& a, int num_sms, size_t max_smem, cudaStream_t stream);

@@ -104,16 +104,28 @@ int linear_q4(const char* what, void* out, int out_dtype, const void* inp, int i
     // bits instead of rounding it, 1.8e-8 of the sum per 16 products (512 tokens, K = 18944: 2.2e-5 off, where
     // fp32 sums in another order are 2e-6 off and the streaming kernel's 3e-7); half an fp16 step is 2^-12.
     const bool gemm = (M > 16 || (M > 8 && M * K > 200 * 1024)) && (out_dtype == B200Q8_F16 || K <= 512);
-    cudaError_t e;
-    if (gemm && q4_gemm_tc_supports(a)) {
+    // Rows that the fast kernels do not take are copied into ones that they do, but for the small: then the generic
+    // kernel is as quick as the copies' launches (1 x 896 x 255 4.7 us, copied 5.8; 4 x 896 x 255 6.9, 6.0; 100 x 300 x 77
+    // 6.2, 13; 1 x 896 x 895 9.8, 6.4; 512 x 3584 x 3583 4611, 43).
+    const bool small = (K < 192 || K * (M < 8 ? M : 8) < 768) && M * N * K < ((size_t)1 << 23);
+    const size_t pad = small ? 0 : q4_pad_bytes(a);
+    Q4Args fast = a;  // as it will be after the copying
+    if (pad) fast.q4 = nullptr, fast.x = nullptr, fast.K = (K + 31) / 32 * 32;
+    const bool use_gemm = gemm && q4_gemm_tc_supports(fast);
+    if (use_gemm || pad) {
         size_t ws = 0, counters = 0, act = 0;
-        q4_gemm_tc_scratch_need(a, sms, &ws, &counters, &act);
+        if (use_gemm) q4_gemm_tc_scratch_need(fast, sms, &ws, &counters, &act);
+        act = (act + 255) / 256 * 256;
         TcScratch scratch;
-        if ((st = stream_scratch(ws, counters, act, sms, stream, &scratch))) return st;
-        e = launch_q4_gemm_tc(a, sms, scratch, stream);
-        return e == cudaSuccess ? B200Q8_OK : cuda_fail(e, "q4_gemm launch");
+        if ((st = stream_scratch(ws, counters, act + pad, sms, stream, &scratch))) return st;
+        cudaError_t e = pad ? launch_q4_pad(&a, scratch.act + act, sms, stream) : cudaSuccess;
+        if (e != cudaSuccess) return cuda_fail(e, "q4_pad launch");
+        if (use_gemm) {
+            e = launch_q4_gemm_tc(a, sms, scratch, stream);
+            return e == cudaSuccess ? B200Q8_OK : cuda_fail(e, "q4_gemm launch");
+        }
     }
-    e = launch_q4_stream(a, sms, smem, stream);
+    cudaError_t e = launch_q4_stream(a, sms, smem, stream);
     if (e == cudaErrorNotSupported) e = launch_q4_linear_generic(a, stream);
     return e == cudaSuccess ? B200Q8_OK : cuda_fail(e, "q4_linear launch");
 }

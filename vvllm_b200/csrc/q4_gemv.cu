@@ -1018,7 +1018,7 @@ StreamPlan plan_stream(const Q4Args& a, size_t M, int num_sms, size_t max_smem)
 
 bool q4_stream_supports(const Q4Args& a)
 {
-    return a.K % 32 == 0 && (uintptr_t)a.q4 % 16 == 0 && (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.scales % 4 == 0 &&
+    return a.K % 32 == 0 && (uintptr_t)a.q4 % 16 == 0 && (uintptr_t)a.x % 16 == 0 &&
            a.N <= (size_t)INT32_MAX - 4096 && encode_fn() != nullptr;
 }
 
