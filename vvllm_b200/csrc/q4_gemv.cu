@@ -134,7 +134,8 @@ constexpr uint64_t kWaitNs = 4000000000ull;  // far above any legitimate wait
 
 struct StreamParams {
     Q4Args a;
-    int M;            // tokens of this launch
+    int M;            // tokens of this launch, `tokens` of them to blockIdx.y
+    int tokens;
     int wk, wk_log2;  // warps per tile
     int stages;       // items in flight per warp
     int nch;          // items per row
@@ -250,7 +251,7 @@ __device__ __forceinline__ int column_of(int m, int d, int M)  // where it is st
     return NT == 1 ? 3 * m + d : d * M + m;
 }
 
-// Tokens into shared memory, `blocks` (a multiple of 8) 32-blocks from block0:
+// Tokens m0 .. m0 + M - 1 into shared memory, `blocks` (a multiple of 8) 32-blocks from block0:
 //   xs      [column][pair of blocks][quarter t][2 blocks] of 8 bytes: the bytes that lane t multiplies
 //           with its word of a block, elements 0 2 4 6 1 3 5 7.  Within a group of W = group / 32 blocks, word
 //           w of lane t starts at element (t * W + w) * 8.  Zero behind K.
@@ -260,7 +261,7 @@ __device__ __forceinline__ int column_of(int m, int d, int M)  // where it is st
 // called once the first loads are under way, `arrived` once they are there.
 template <int NT, bool kF16, class Asked, class Arrived>
 __device__ __forceinline__ bool stage_tokens(unsigned char* xs, float* weight, unsigned char* direct,
-                                             const StreamParams& p, int W, int block0, int blocks, Asked asked, Arrived arrived)
+                                             const StreamParams& p, int m0, int M, int W, int block0, int blocks, Asked asked, Arrived arrived)
 {
     constexpr int U = 5;  // chunks whose loads are in flight
     constexpr int kRaw = kF16 ? 4 : 8;
@@ -272,7 +273,7 @@ __device__ __forceinline__ bool stage_tokens(unsigned char* xs, float* weight, u
     unsigned char* const dst0 = xs + (ub >> 1) * 64 + (o / W) * 16 + (ub & 1) * 8;
     bool any = false, first = true;
     // Rounds: every half warp a chunk of one token, chunks c0 + half.
-    for (int m = 0, c0 = 0; m < p.M;) {
+    for (int m = 0, c0 = 0; m < M;) {
         uint32_t raw[U][kRaw];
         int lm = m, lc = c0;
 #pragma unroll
@@ -280,9 +281,9 @@ __device__ __forceinline__ bool stage_tokens(unsigned char* xs, float* weight, u
             const int k = block0 * 32 + (lc + half) * 128 + u * 8;
 #pragma unroll
             for (int j = 0; j < kRaw; j++) raw[q][j] = 0;
-            if (lm < p.M && lc + half < chunks && k < K) {
+            if (lm < M && lc + half < chunks && k < K) {
                 const uint4* src = reinterpret_cast<const uint4*>(static_cast<const char*>(p.a.x) +
-                                                                  ((size_t)lm * K + k) * (kF16 ? 2 : 4));
+                                                                  ((size_t)(m0 + lm) * K + k) * (kF16 ? 2 : 4));
 #pragma unroll
                 for (int j = 0; j < kRaw / 4; j++) {
                     const uint4 r = src[j];
@@ -295,7 +296,7 @@ __device__ __forceinline__ bool stage_tokens(unsigned char* xs, float* weight, u
         if (first) asked();
 #pragma unroll
         for (int q = 0; q < U; q++) {
-            if (m >= p.M) break;  // uniform in the CTA
+            if (m >= M) break;  // uniform in the CTA
             // The largest |x| as bits: above every number for an infinity or NaN.
             float v[8];
             uint32_t top;
@@ -345,7 +346,7 @@ __device__ __forceinline__ bool stage_tokens(unsigned char* xs, float* weight, u
                         const uint32_t hi = __byte_perm(y[4 + h], y[6 + h], n == 2 ? 0x0062 : 0x5140);
                         d[h] = __byte_perm(lo, hi, n == 1 ? 0x7632 : 0x5410) ^ 0x80808080u;
                     }
-                    *reinterpret_cast<uint2*>(dst + column_of<NT>(m, n, p.M) * cs) = make_uint2(d[0], d[1]);
+                    *reinterpret_cast<uint2*>(dst + column_of<NT>(m, n, M) * cs) = make_uint2(d[0], d[1]);
                 }
                 if (u < (NT == 1 ? 3 : 1))
                     weight[c * 8 + (NT == 1 ? 3 * m + u : m)] = __uint_as_float((uint32_t)(e - 22 - 4 + 8 * u + 127) << 23);
@@ -362,7 +363,7 @@ __device__ __forceinline__ bool stage_tokens(unsigned char* xs, float* weight, u
 // fp16 tokens as they are: [column m][block][quarter t] of eight, elements 0 4 1 5 2 6 3 7 of the word that lane t
 // multiplies with its word of the block (the words in the order above).  Zero behind K.
 template <class Asked, class Arrived>
-__device__ __forceinline__ void stage_halves(unsigned char* xs, const StreamParams& p, int W, int block0, int blocks, Asked asked,
+__device__ __forceinline__ void stage_halves(unsigned char* xs, const StreamParams& p, int m0, int M, int W, int block0, int blocks, Asked asked,
                                              Arrived arrived)
 {
     constexpr int U = 8;  // chunks whose loads are in flight
@@ -372,22 +373,22 @@ __device__ __forceinline__ void stage_halves(unsigned char* xs, const StreamPara
     const int o = u & (4 * W - 1), ub = u / (4 * W) * W + (o & (W - 1));
     unsigned char* const dst0 = xs + ub * 64 + (o / W) * 16;
     bool first = true;
-    for (int m = 0, c0 = 0; m < p.M;) {
+    for (int m = 0, c0 = 0; m < M;) {
         uint4 raw[U];
         int lm = m, lc = c0;
 #pragma unroll
         for (int q = 0; q < U; q++) {
             const int k = block0 * 32 + (lc + half) * 128 + u * 8;
             raw[q] = make_uint4(0, 0, 0, 0);
-            if (lm < p.M && lc + half < chunks && k < K)
-                raw[q] = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.a.x) + (size_t)lm * K + k);
+            if (lm < M && lc + half < chunks && k < K)
+                raw[q] = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.a.x) + (size_t)(m0 + lm) * K + k);
             lc += halves;
             if (lc >= chunks) lc = 0, lm++;
         }
         if (first) asked();
 #pragma unroll
         for (int q = 0; q < U; q++) {
-            if (m >= p.M) break;  // uniform in the CTA
+            if (m >= M) break;  // uniform in the CTA
             const uint4 r = raw[q];
             const uint4 v = make_uint4(__byte_perm(r.x, r.z, 0x5410), __byte_perm(r.x, r.z, 0x7632),
                                        __byte_perm(r.y, r.w, 0x5410), __byte_perm(r.y, r.w, 0x7632));
@@ -465,6 +466,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     const cg::cluster_group cluster = cg::this_cluster();
     const int csize = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int warps = blockDim.x >> 5;
+    const int m0 = (int)blockIdx.y * p.tokens, M = min(p.tokens, p.M - m0);  // this CTA's tokens
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) &
                                                            ~static_cast<uintptr_t>(1023));
@@ -473,7 +475,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     unsigned char* xs = reinterpret_cast<unsigned char*>(bars + warps * kMaxStages);
     const int xchunks = p.per * C::kChunks;
     const size_t cs = column_stride(xchunks * 4, kHalves);
-    float* weight = reinterpret_cast<float*>(xs + (kHalves ? 1 : 3) * p.M * cs);
+    float* weight = reinterpret_cast<float*>(xs + (kHalves ? 1 : 3) * M * cs);
     float* red = weight + xchunks * C::kCols;         // [buffer][warp][tile's outputs]
     float* cbuf = red + C::red_bufs(p.wk, csize) * warps * C::kSums;  // [2][rank][group][tile's outputs] of a cluster's CTAs (in rank 0)
     unsigned char* direct = reinterpret_cast<unsigned char*>(cbuf + (csize > 1 ? 2 * csize * (warps >> p.wk_log2) * C::kSums : 0));
@@ -519,7 +521,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     }
     pdl_wait();
     pdl_launch_dependents();
-    const uint64_t policy = tc::l2_policy_evict_first();
+    const uint64_t policy = gridDim.y == 1 ? tc::l2_policy_evict_first() : tc::l2_policy_evict_normal();
     auto load_item = [&](int stage) {
         tc::mbar_arrive_expect_tx(bar0 + 8 * stage, kItemBytes);
 #pragma unroll
@@ -592,13 +594,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     };
     bool any_direct = false;
     if constexpr (kHalves) {
-        stage_halves(xs, p, W, ch0 * C::kChunks * 4, xchunks * 4, asked, arrived);
+        stage_halves(xs, p, m0, M, W, ch0 * C::kChunks * 4, xchunks * 4, asked, arrived);
         __syncthreads();
     } else {
         const int block0 = ch0 * C::kChunks * 4, blocks = xchunks * 4;
         any_direct = __syncthreads_or(p.a.in_dtype == kF16
-                                          ? stage_tokens<NT, true>(xs, weight, direct, p, W, block0, blocks, asked, arrived)
-                                          : stage_tokens<NT, false>(xs, weight, direct, p, W, block0, blocks, asked, arrived));
+                                          ? stage_tokens<NT, true>(xs, weight, direct, p, m0, M, W, block0, blocks, asked, arrived)
+                                          : stage_tokens<NT, false>(xs, weight, direct, p, m0, M, W, block0, blocks, asked, arrived));
     }
     if (csize > 1) cluster.sync();  // every rank runs before rank 0's memory is stored to
 
@@ -606,9 +608,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
         xoff[nt] = tc::smem_u32(xs) + t * 16 +
-                   (uint32_t)((kHalves   ? min(nt * 8 + g, p.M - 1)
-                               : NT == 1 ? min(g, 3 * p.M - 1)
-                                         : nt * p.M + min(g, p.M - 1)) * cs);
+                   (uint32_t)((kHalves   ? min(nt * 8 + g, M - 1)
+                               : NT == 1 ? min(g, 3 * M - 1)
+                                         : nt * M + min(g, M - 1)) * cs);
     // The lane's words of group 0 of a box: 16-byte piece ((t * W) / 4) ^ row of its row; another group is an
     // XOR away.
     const uint32_t wlane = row * 128 + ((((t * W) >> 2) ^ row) << 4) + ((t * W) & 3) * 4;
@@ -759,12 +761,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
             v[0][2] = t == 0 ? v[0][2] + v[0][3] + b : d + v[0][2] + v[0][3];
         }
         auto mine = [&](int o, int i) {  // whether v[o][i] is an output's sum
-            return kOneTile ? (t & 1) == 0 && (i & 1) == 0 && mt < p.M : 8 * o + mt + (i & 1) < p.M;
+            return kOneTile ? (t & 1) == 0 && (i & 1) == 0 && mt < M : 8 * o + mt + (i & 1) < M;
         };
         auto put = [&](int m, int r, float y) {
             const long long n = (long long)tile * 16 + r;
             if (n >= N) return;
-            const long long o = (long long)m * N + n;
+            const long long o = (long long)(m0 + m) * N + n;
             if (p.a.out_dtype == kF16)
                 q4_store<__half>(static_cast<__half*>(p.a.out) + o,
                                  p.a.res ? static_cast<const __half*>(p.a.res) + o : nullptr, y, p.a.bias, n);
@@ -790,15 +792,15 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
                 if (mine(o, i)) wsum[(8 * o + mt + (i & 1)) * 16 + row + 8 * (i >> 1)] = v[o][i];
         if (any_direct && tile < p.tiles) {  // rare: infinities or NaN among this CTA's elements
             __syncwarp();
-            for (int m = 0; m < p.M; m++)
+            for (int m = 0; m < M; m++)
                 for (int c = kw; c < xchunks; c += wk)
-                    if (direct[m * xchunks + c]) direct_chunk(p.a, wsum + m * 16, tile, m, ch0 * C::kChunks + c);
+                    if (direct[m * xchunks + c]) direct_chunk(p.a, wsum + m * 16, tile, m0 + m, ch0 * C::kChunks + c);
         }
         if (wk == 1)
             __syncwarp();
         else
             asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(wk * 32) : "memory");
-        const int gt = kw * 32 + lane, outs = p.M * 16;
+        const int gt = kw * 32 + lane, outs = M * 16;
         const float* gsum = rbuf + group * wk * C::kSums;
         auto warp_sums = [&](int e) {
             float y = gsum[e];
@@ -880,7 +882,7 @@ cudaError_t launch_stream(const StreamParams& p, const StreamPlan& s, int num_sm
     const int groups = s.warps / p.wk;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3((unsigned)s.warps * 32);
-    cfg.dynamicSmemBytes = C::smem(s.warps, p.stages, p.M, p.per, s.cluster, p.wk);
+    cfg.dynamicSmemBytes = C::smem(s.warps, p.stages, p.tokens, p.per, s.cluster, p.wk);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -917,7 +919,18 @@ cudaError_t launch_stream(const StreamParams& p, const StreamPlan& s, int num_sm
         }
         resident = std::max(1, known[i].n);
     }
-    cfg.gridDim = dim3((unsigned)(std::min((p.tiles + groups - 1) / groups, resident) * s.cluster));
+    // Of several passes over the weights those that fit run side by side, and a CTA puts its tokens into shared
+    // memory once for all its tiles: as many per pass as end soonest (the tokens count as two rounds of tiles).
+    const int passes = (p.M + p.tokens - 1) / p.tokens, turns = (p.tiles + groups - 1) / groups;
+    int wide = std::min(turns, resident);
+    if (passes > 1) {
+        double best = 1e30;
+        for (int g = wide; g >= 1; g--) {
+            const double cost = (double)(((long long)g * passes + resident - 1) / resident) * ((turns + g - 1) / g + 2);
+            if (cost < best) best = cost, wide = g;
+        }
+    }
+    cfg.gridDim = dim3((unsigned)(wide * s.cluster), (unsigned)passes);
     e = cudaLaunchKernelEx(&cfg, kern, mw, p);
     if (e == cudaSuccess) note_launch();
     return e;
@@ -963,9 +976,9 @@ constexpr int kMaxCluster = 8;
 // is what a CTA of few tiles spends its time on, so a long K is split over as many SMs as the tiles
 // leave free (8 tokens in bytes, 896 x 4864: 9.6 us on clusters of two, 12 without), and over more where
 // that leaves warps less to do (9 tokens, 14336 x 8192: 32 us in clusters of two, in single CTAs 48).
-StreamPlan plan_stream(const Q4Args& a, size_t M, int num_sms, size_t max_smem)
+StreamPlan plan_stream(const Q4Args& a, size_t M, long long passes, int num_sms, size_t max_smem)
 {
-    const long long tiles = (long long)((a.N + 15) / 16);
+    const long long tiles = (long long)((a.N + 15) / 16) * passes;
     const bool f16 = a.in_dtype == kF16;
     for (int m = (int)std::min<size_t>(M, f16 ? kMaxTokens : kMaxDigitTokens); m >= 1; m--) {
         const bool halves = f16 && m > 2;
@@ -1026,17 +1039,19 @@ cudaError_t launch_q4_stream(const Q4Args& a, int num_sms, size_t max_smem, cuda
 {
     if (!q4_stream_supports(a)) return cudaErrorNotSupported;
     const size_t ib = a.in_dtype == kF16 ? 2 : 4, ob = a.out_dtype == kF16 ? 2 : 4;
-    const StreamPlan first = plan_stream(a, a.M, num_sms, max_smem);
-    if (!first.tokens) return cudaErrorNotSupported;  // one token's slice exceeds the shared memory
+    const StreamPlan most = plan_stream(a, a.M, 1, num_sms, max_smem);
+    if (!most.tokens) return cudaErrorNotSupported;  // one token's slice exceeds the shared memory
+    // Passes of as good as equal numbers of tokens, up to 32768 of them to a launch.
+    const size_t passes = (a.M + most.tokens - 1) / most.tokens, tokens = (a.M + passes - 1) / passes;
+    const StreamPlan s = passes == 1 ? most : plan_stream(a, tokens, (long long)passes, num_sms, max_smem);
     for (size_t m0 = 0; m0 < a.M;) {
-        const size_t left = a.M - m0;
-        const StreamPlan s = left >= (size_t)first.tokens ? first : plan_stream(a, left, num_sms, max_smem);
         StreamParams p;
         p.a = a;
         p.a.x = static_cast<const char*>(a.x) + m0 * a.K * ib;
         p.a.out = static_cast<char*>(a.out) + m0 * a.N * ob;
         p.a.res = a.res ? static_cast<const char*>(a.res) + m0 * a.N * ob : nullptr;
-        p.M = s.tokens;
+        p.tokens = s.tokens;
+        p.M = (int)std::min(a.M - m0, (size_t)s.tokens * 32768);
         p.wk = s.wk;
         p.wk_log2 = s.wk == 16 ? 4 : s.wk == 8 ? 3 : s.wk == 4 ? 2 : s.wk == 2 ? 1 : 0;
         p.stages = s.stages;
@@ -1047,7 +1062,7 @@ cudaError_t launch_q4_stream(const Q4Args& a, int num_sms, size_t max_smem, cuda
                         : a.group == 64 ? launch_stream_nt<64>(p, s, num_sms, max_smem, stream)
                                         : launch_stream_nt<128>(p, s, num_sms, max_smem, stream);
         if (e != cudaSuccess) return e;
-        m0 += (size_t)s.tokens;
+        m0 += (size_t)p.M;
     }
     return cudaSuccess;
 }
