@@ -95,19 +95,22 @@ int linear_q4(const char* what, void* out, int out_dtype, const void* inp, int i
     a.group = group;
     a.in_dtype = in_dtype;
     a.out_dtype = out_dtype;
-    // Up to 16 fp16 tokens (8 in fp32) the streaming kernel reads the weights once; above, once for every so many,
-    // where the GEMM (fp16 tokens) reads them once at a rate bound by its dequantization.  Measured on B200,
-    // streaming vs GEMM: 37888 x 3584 at 16 tokens 24 vs 38 us, at 17 38 vs 38, at 32 48 vs 38; 896 x 4864 at 16 8 vs
-    // 24.  Tokens that need clusters of eight are slower: 3584 x 18944 at 9 24 vs 28, at 16 38 vs 28;
+    // The streaming kernel goes over the weights once for every 16 fp16 tokens (8 in fp32), in passes that run side by
+    // side; the GEMM (fp16 tokens) once, at a rate bound by its dequantization and with a start of its own.
+    // Measured on B200, streaming vs GEMM: 37888 x 3584 at 16 tokens 24 vs 38 us, at 17 39 vs 38; 3584 x 3584 at 64 16
+    // vs 21, at 128 25 vs 24; 896 x 4864 at 64 12 vs 26, at 256 26 vs 25; 4864 x 896 at 32 9 vs 10, at 64 11 vs 10.
+    // Up to 16 tokens only those that need clusters of eight are slower: 3584 x 18944 at 9 24 vs 28, at 16 38 vs 28;
     // 8192 x 28672 at 8 38 vs 64, at 9 72 vs 64.
+    const size_t work = M * N * K;
+    bool gemm = M > 16 ? work > (K < 2048 ? (size_t)1 << 28 : (size_t)1 << 30) : M > 8 && M * K > 200 * 1024 && work > ((size_t)1 << 29);
     // fp32 outputs take the GEMM only with short sums: the tensor core's accumulator drops what falls below its 24
     // bits instead of rounding it, 1.8e-8 of the sum per 16 products (512 tokens, K = 18944: 2.2e-5 off, where
     // fp32 sums in another order are 2e-6 off and the streaming kernel's 3e-7); half an fp16 step is 2^-12.
-    const bool gemm = (M > 16 || (M > 8 && M * K > 200 * 1024)) && (out_dtype == B200Q8_F16 || K <= 512);
+    gemm = gemm && (out_dtype == B200Q8_F16 || K <= 512);
     // Rows that the fast kernels do not take are copied into ones that they do, but for the small: then the generic
     // kernel is as quick as the copies' launches (1 x 896 x 255 4.7 us, copied 5.8; 4 x 896 x 255 6.9, 6.0; 100 x 300 x 77
     // 6.2, 13; 1 x 896 x 895 9.8, 6.4; 512 x 3584 x 3583 4611, 43).
-    const bool small = (K < 192 || K * (M < 8 ? M : 8) < 768) && M * N * K < ((size_t)1 << 23);
+    const bool small = (K < 192 || K * (M < 8 ? M : 8) < 768) && work < ((size_t)1 << 23);
     const size_t pad = small ? 0 : q4_pad_bytes(a);
     Q4Args fast = a;  // as it will be after the copying
     if (pad) fast.q4 = nullptr, fast.x = nullptr, fast.K = (K + 31) / 32 * 32;
