@@ -81,7 +81,7 @@ cudaError_t launch_generic(const Q4Args& a, cudaStream_t stream)
 
 
 // ----------------------------------------------------------------------------------------------
-// Streaming kernel: K % 32 == 0, aligned pointers, up to 16 tokens (8 in fp32).
+// Streaming kernel: K % 32 == 0, aligned pointers, up to 16 tokens (8 in fp32) to a CTA and pass over the weights.
 //
 // Three to sixteen fp16 tokens: the codes become the integers q in fp16 (nine operations per eight), and
 // mma.sync m16n8k16 multiplies them with the tokens as they are; products are exact, the tensor core sums a
