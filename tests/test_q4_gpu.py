@@ -313,3 +313,13 @@ def test_linear_bad_tokens_stay_in_their_row_when_copied(cuda, M):
         y = u.linear(x, q, s, 64)
     assert np.array_equal(got[1:-1], y[1:-1].astype(np.float32)) and np.isnan(got[-1]).all()
     assert np.array_equal(np.isfinite(got[0]), np.isfinite(y[0]))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("N,K", [(7, 288), (5, 1000), (33, 40), (9, 72), (64, 1016), (300, 8), (40, 2320), (1, 3544)])
+def test_quantize_rows_that_end_within_a_group(cuda, N, K, group, bf16):
+    """Rows of whole octets: the last group is short, and the next row starts a new one."""
+    w = make_weight(N, K, N + 5 * K)
+    w[:, -1] = 3.0  # the short group's largest weight is its last
+    _check_quantize(cuda, u.round_to_bf16(w).astype(np.float32) if bf16 else w, group, bf16)

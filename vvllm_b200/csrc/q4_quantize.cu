@@ -14,6 +14,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -101,30 +102,42 @@ __device__ __forceinline__ void load8(const uint16_t* p, float2* v)
     for (int i = 0; i < 4; i++) v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
 }
 
-// Whole groups (K % group == 0), aligned: the matrix as one run of octets of weights.  A thread takes O
+// Aligned rows of octets (K % 8 == 0): the matrix as one run of octets of weights; kShort: rows end within a
+// group, and threads stand for the missing octets, `per_row` runs of octets to a row in all.  A thread takes O
 // consecutive octets (16 bytes of bf16 or 32 of fp32 each), neighbouring threads a group, and U such
 // runs at a time.  bf16 takes two octets a thread: a group's scale is then worked out by half as many.
 // The quotients are IEEE's without a division per weight: with y = 1 / s rounded to nearest, t = w y and the
 // exact remainder w - t s, t + (w - t s) y is the correctly rounded w / s (Markstein), in packed
 // operations; adding 1.5 * 2^23 then rounds it to an integer, ties to even.  Groups whose 1 / s is no normal
 // number and NaN weights take the plain way.
-// Bound by HBM for fp32 (18944 x 3584: 48 us, 6.4 TB/s), by instruction issue for bf16.
-template <typename WT, int G, int O, int U>
+// Bound by HBM for fp32 (18944 x 3584: 44 us, 6.9 TB/s), by HBM and instruction issue for bf16 (37888 x 3584: 56 us);
+// rows that end within a group 26316 x 2592 57 us in fp32, 48 in bf16 (the generic kernel: 200).
+template <typename WT, int G, int O, int U, bool kShort>
 __global__ void __launch_bounds__(256) q4_quantize_flat_kernel(const WT* __restrict__ w, uint32_t* __restrict__ q4,
-                                                               uint16_t* __restrict__ scales, long long runs)
+                                                               uint16_t* __restrict__ scales, long long runs, int per_row, int K)
 {
     constexpr int kLanes = G / (8 * O);  // threads of a group
+    // Where run r's weights lie, in runs; false: behind its row's end.
+    auto find = [&](long long r, long long& at) {
+        at = r;
+        if (!kShort) return r < runs;
+        const long long row = r / per_row;
+        const int c = (int)(r - row * per_row), have = K / (8 * O);
+        at = row * have + c;
+        return r < runs && c < have;
+    };
     pdl_wait();
     pdl_launch_dependents();
     const long long base = (long long)blockIdx.x * (256 * U) + threadIdx.x;
     float2 v[U][4 * O];
 #pragma unroll
     for (int i = 0; i < U; i++) {
-        const long long r = base + i * 256;
+        long long at;
+        const bool in = find(base + i * 256, at);
 #pragma unroll
         for (int o = 0; o < O; o++)
-            if (r < runs)
-                load8(w + (r * O + o) * 8, v[i] + 4 * o);
+            if (in)
+                load8(w + (at * O + o) * 8, v[i] + 4 * o);
             else
                 v[i][4 * o] = v[i][4 * o + 1] = v[i][4 * o + 2] = v[i][4 * o + 3] = make_float2(0.0f, 0.0f);
     }
@@ -168,11 +181,12 @@ __global__ void __launch_bounds__(256) q4_quantize_flat_kernel(const WT* __restr
                     code[o] |= q4_code(v[i][4 * o + j].x, s) << (8 * j) | q4_code(v[i][4 * o + j].y, s) << (8 * j + 4);
             }
         }
-        if (r < runs) {
+        long long at;
+        if (find(r, at)) {  // (a group's first octet is there)
             if constexpr (O == 2)
-                __stcs(reinterpret_cast<uint2*>(q4) + r, make_uint2(code[0], code[1]));
+                __stcs(reinterpret_cast<uint2*>(q4) + at, make_uint2(code[0], code[1]));
             else
-                __stcs(q4 + r, code[0]);
+                __stcs(q4 + at, code[0]);
             if (threadIdx.x % kLanes == 0) scales[r / kLanes] = (uint16_t)bits;
         }
     }
@@ -299,14 +313,24 @@ cudaError_t quantize_typed(const WT* w, size_t N, size_t K, int group, uint8_t* 
                            cudaStream_t stream)
 {
     const long long ng = (long long)((K + group - 1) / group), groups = ng * (long long)N;
-    constexpr int O = sizeof(WT) == 2 ? 2 : 1, U = 2;
-    if (K % group == 0 && aligned(w, 16) && aligned(q4, 4 * O)) {
-        const long long runs = groups * (group / (8 * O));
+    auto flat = [&](auto octets, auto short_rows) {
+        constexpr int O = decltype(octets)::value, U = 2;
+        constexpr bool kShort = decltype(short_rows)::value;
+        const long long per_row = ng * (group / (8 * O)), runs = per_row * (long long)N;
         const dim3 grid((unsigned)((runs + 256 * U - 1) / (256 * U)));
-        uint32_t* words = reinterpret_cast<uint32_t*>(q4);
-        if (group == 32) return launch_pdl(q4_quantize_flat_kernel<WT, 32, O, U>, grid, dim3(256), stream, w, words, scales, runs);
-        if (group == 64) return launch_pdl(q4_quantize_flat_kernel<WT, 64, O, U>, grid, dim3(256), stream, w, words, scales, runs);
-        return launch_pdl(q4_quantize_flat_kernel<WT, 128, O, U>, grid, dim3(256), stream, w, words, scales, runs);
+        auto go = [&](auto kern) {
+            return launch_pdl(kern, grid, dim3(256), stream, w, reinterpret_cast<uint32_t*>(q4), scales, runs, (int)per_row, (int)K);
+        };
+        return group == 32   ? go(q4_quantize_flat_kernel<WT, 32, O, U, kShort>)
+               : group == 64 ? go(q4_quantize_flat_kernel<WT, 64, O, U, kShort>)
+                             : go(q4_quantize_flat_kernel<WT, 128, O, U, kShort>);
+    };
+    constexpr int O = sizeof(WT) == 2 ? 2 : 1;
+    using One = std::integral_constant<int, 1>;
+    if (K % 8 == 0 && aligned(w, 16) && aligned(q4, 4 * O)) {
+        if (K % group == 0) return flat(std::integral_constant<int, O>(), std::false_type());
+        if (O == 2 && K % 16 == 0) return flat(std::integral_constant<int, O>(), std::true_type());
+        return flat(One(), std::true_type());
     }
     const long long blocks = std::min<long long>((groups + 7) / 8, (long long)num_sms * 64);
     q4_quantize_generic_kernel<WT><<<(unsigned)blocks, 256, 0, stream>>>(w, q4, scales, groups, (int)ng, (long long)K,
