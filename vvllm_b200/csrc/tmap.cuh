@@ -12,27 +12,38 @@
 #include <stdint.h>
 #include <string.h>
 
-#include <mutex>
-
 namespace b200q8 {
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+typedef CUresult (*CtxGetCurrentFn)(CUcontext*);
+
+inline void* driver_entry(const char* name)
+{
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    const bool found = cudaGetDriverEntryPoint(name, &ptr, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+    cudaGetLastError();
+    return found ? ptr : nullptr;
+}
+
 inline EncodeTiledFn encode_fn()
 {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(ptr);
-        cudaGetLastError();
-    });
+    static const EncodeTiledFn fn = reinterpret_cast<EncodeTiledFn>(driver_entry("cuTensorMapEncodeTiled"));
     return fn;
+}
+
+// The encoder needs a context, and a host thread whose first CUDA call this is has none yet (asking for the
+// device's number binds none): the current device's primary context, as a launch would bind it.
+inline bool bind_context()
+{
+    static const CtxGetCurrentFn current = reinterpret_cast<CtxGetCurrentFn>(driver_entry("cuCtxGetCurrent"));
+    CUcontext ctx = nullptr;
+    if (current && current(&ctx) == CUDA_SUCCESS && ctx) return true;
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
 }
 
 struct TmapDesc {
@@ -61,7 +72,7 @@ inline bool tmap_2d(CUtensorMap* out, const TmapDesc& d)
             return true;
         }
     EncodeTiledFn enc = encode_fn();
-    if (!enc) return false;
+    if (!enc || !bind_context()) return false;
     const cuuint64_t dims[2] = {(cuuint64_t)d.inner, (cuuint64_t)d.outer};
     const cuuint64_t strides[1] = {(cuuint64_t)d.row_bytes};
     const cuuint32_t box[2] = {d.box_inner, d.box_outer};
