@@ -62,6 +62,9 @@ B200Q8_API uint64_t b200q8_launch_count(void);
 /* ------------------------------------------------------------------------
  * 1. Kernel layer.  All pointers are device pointers; work is enqueued on
  *    `stream` and the call returns without synchronising.
+ *    Any number of host threads may call, on streams of their own or on one: a call's launches
+ *    stay together on its stream.  What a stream's calls share belongs to its handle (for
+ *    cudaStreamPerThread, to the thread's stream): let its work end before the stream is destroyed.
  * ------------------------------------------------------------------------ */
 
 /* q[N,K], scales[N] = per-row absmax int8 quantization of w[N,K] (fp32).
@@ -123,8 +126,8 @@ B200Q8_API int b200q8_linear_q8_ex(void* out, int out_dtype, const void* inp, in
  * larger shapes return B200Q8_ERR_UNSUPPORTED.  The first call on a device looks
  * up the array's device address; make that first call before any stream
  * capture.  All calls share the array, which keeps the last call's contents
- * (each call clears the counters it needs); calls that overlap on one GPU race
- * on it and must be serialised by the caller. */
+ * (each call clears the counters it needs); calls whose work overlaps on one GPU (on
+ * different streams) race on it and must be serialised by the caller. */
 B200Q8_API int b200q8_linear_q8_noalloc(void* out, int out_dtype, const void* inp, int in_dtype,
                                         const int8_t* weight, const float* scales, const float* bias,
                                         const void* residual, size_t M, size_t N, size_t K,

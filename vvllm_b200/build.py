@@ -24,7 +24,7 @@ LIB = os.path.join(HERE, "libb200q8.so")
 SOURCES = ["b200q8_api.cu", "q8_gemv.cu", "q8_quantize.cu", "q8_gemm_tc.cu", "q8_gemv_tc.cu", "gather.cu", "prologue.cu", "q8st.cu",
            "q4_api.cu", "q4_pad.cu", "q4_quantize.cu", "q4_gemv.cu", "logits.cu"]
 HEADERS = ["common.cuh", "kernels.h", "tc_utils.cuh", "sk_common.cuh", "tmap.cuh", "prologue.cuh", "p2p.cuh",
-           "q4_common.cuh"]
+           "q4_common.cuh", "stream_order.h"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # No --use_fast_math / -ftz: the quantize kernel must keep denormals and IEEE division.

@@ -93,21 +93,10 @@ bool valid_dtype(int d) { return d == B200Q8_F32 || d == B200Q8_F16; }
 
 // Stream-K scratch of the tensor-core GEMM, one per (device, stream): launches
 // on one stream are ordered, so they may share it; different streams may run
-// concurrently, so they do not.  Allocated on first use (outside any graph
-// capture) and grown when a larger shape needs more; never shrunk.
-struct ScratchKey {
-    int dev;
-    cudaStream_t stream;
-    bool operator==(const ScratchKey& o) const { return dev == o.dev && stream == o.stream; }
-};
-struct ScratchKeyHash {
-    size_t operator()(const ScratchKey& k) const
-    {
-        return std::hash<uintptr_t>()((uintptr_t)k.stream) * 31u + (size_t)k.dev;
-    }
-};
-std::mutex g_scratch_mu;
-std::unordered_map<ScratchKey, TcScratch, ScratchKeyHash> g_scratch;
+// concurrently, so they do not.  Host threads that call on one stream take turns:
+// a call holds the stream's entry from here to its last launch.  Allocated on first use (outside
+// any graph capture) and grown when a larger shape needs more; never shrunk.
+PerStream<TcScratch>& g_scratch = *new PerStream<TcScratch>;  // never destroyed: threads may still call at exit
 
 struct ScratchNeed {
     size_t ws = 0, counters = 0, exps = 0, act = 0;
@@ -138,13 +127,14 @@ int grow(T** buf, size_t* have, size_t need, size_t dflt, cudaStream_t stream, b
     return B200Q8_OK;
 }
 
-int get_scratch(const ScratchNeed& need, int num_sms, cudaStream_t stream, TcScratch* out)
+// The scratch of (current device, stream), which `hold` keeps for the caller while it lives.
+int get_scratch(const ScratchNeed& need, int num_sms, cudaStream_t stream, ScratchHold* hold, TcScratch* out)
 {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-    std::lock_guard<std::mutex> lk(g_scratch_mu);
-    TcScratch& s = g_scratch[ScratchKey{dev, stream}];
+    g_scratch.hold(stream_key(dev, stream, cudaStreamPerThread), hold);
+    TcScratch& s = **hold;
     // Default capacities: 128-column partials on every SM, 64K tiles.
     int st;
     if ((st = grow(&s.ws, &s.ws_floats, need.ws, (size_t)2 * num_sms * 128 * 128, stream, false, "partials")) ||
@@ -166,10 +156,9 @@ int get_scratch(const ScratchNeed& need, int num_sms, cudaStream_t stream, TcScr
 // graph (and what is instantiated from it) through a user object; when the last of them is destroyed the
 // set goes back to be taken by a later capture.  Never destroyed, as graphs may outlive this library's statics.
 struct CaptureScratch {
-    int dev = 0;
     bool taken = false;
     unsigned long long capture = 0;  // whose calls on `stream` it serves
-    cudaStream_t stream = nullptr;
+    StreamKey stream;
     TcScratch s;
 };
 std::mutex& g_capture_mu = *new std::mutex;  // not held during CUDA calls: a release may come from within one
@@ -211,8 +200,7 @@ int fill_capture_scratch(const ScratchNeed& need, bool fresh, TcScratch* s)
     return st;
 }
 
-int capture_scratch(ScratchNeed need, int dev, cudaStream_t stream, unsigned long long capture, cudaGraph_t graph,
-                    TcScratch* out)
+int capture_scratch(ScratchNeed need, const StreamKey& stream, unsigned long long capture, cudaGraph_t graph, TcScratch* out)
 {
     // In powers of two, so that a later capture finds one that fits.
     for (size_t* n : {&need.ws, &need.counters, &need.act}) {
@@ -224,7 +212,7 @@ int capture_scratch(ScratchNeed need, int dev, cudaStream_t stream, unsigned lon
     {
         std::lock_guard<std::mutex> lk(g_capture_mu);
         for (CaptureScratch* i : g_capture) {
-            if (i->dev != dev || !holds(i->s, need)) continue;
+            if (i->stream.dev != stream.dev || !holds(i->s, need)) continue;
             if (i->taken && i->capture == capture && i->stream == stream) {
                 *out = i->s;
                 return B200Q8_OK;
@@ -240,7 +228,6 @@ int capture_scratch(ScratchNeed need, int dev, cudaStream_t stream, unsigned lon
     const bool fresh = !c;
     if (fresh) {
         c = new CaptureScratch;
-        c->dev = dev;
         c->taken = true;
         c->capture = capture;
         c->stream = stream;
@@ -278,22 +265,19 @@ int reset_scratch_counters(int dev)
     {
         std::lock_guard<std::mutex> lk(g_capture_mu);
         for (const CaptureScratch* c : g_capture)
-            if (c->dev == dev) captured.push_back(c->s);
+            if (c->stream.dev == dev) captured.push_back(c->s);
     }
     for (const TcScratch& s : captured) {
         const cudaError_t e = cudaMemset(s.counter_ptr, 0, s.counters * sizeof(int));
         if (e != cudaSuccess) return cuda_fail(e, "reset scratch counters");
     }
-    std::lock_guard<std::mutex> lk(g_scratch_mu);
-    for (auto& kv : g_scratch) {
-        if (kv.first.dev != dev) continue;
-        cudaError_t e = cudaSuccess;
-        if (kv.second.counter_ptr) e = cudaMemset(kv.second.counter_ptr, 0, kv.second.counters * sizeof(int));
-        if (e == cudaSuccess && kv.second.amax)
-            e = cudaMemset(kv.second.amax, 0, (kMaxArgmaxTokens + 1) * sizeof(unsigned long long));
-        if (e != cudaSuccess) return cuda_fail(e, "reset scratch counters");
-    }
-    return B200Q8_OK;
+    cudaError_t e = cudaSuccess;
+    g_scratch.for_each([&](const StreamKey& k, TcScratch& s) {
+        if (k.dev != dev) return;
+        if (e == cudaSuccess && s.counter_ptr) e = cudaMemset(s.counter_ptr, 0, s.counters * sizeof(int));
+        if (e == cudaSuccess && s.amax) e = cudaMemset(s.amax, 0, (kMaxArgmaxTokens + 1) * sizeof(unsigned long long));
+    });
+    return e == cudaSuccess ? B200Q8_OK : cuda_fail(e, "reset scratch counters");
 }
 
 // Weights up to this size with few tokens go to the SIMT GEMV under ALGO_AUTO.
@@ -386,11 +370,12 @@ int linear_impl(void* out, int out_dtype, const void* inp, int in_dtype, const i
         s1.norm_w = norm_w;
         simt_pro = gemv_stream_supports(s1, d.max_smem);
     }
+    ScratchHold hold;  // to the last launch below
     if (pro != kProNone && !use_i8 && !simt_pro) {
         ScratchNeed need;
         need.act = M * K * ib;
         TcScratch scratch;
-        if ((st = get_scratch(need, d.num_sms, stream, &scratch))) return st;
+        if ((st = get_scratch(need, d.num_sms, stream, &hold, &scratch))) return st;
         e = launch_prologue(pro, inp, scratch.act, in_dtype, norm_w, eps, M, K, true, stream);
         if (e != cudaSuccess) return cuda_fail(e, "prologue launch");
         a.x = inp = scratch.act;
@@ -405,7 +390,7 @@ int linear_impl(void* out, int out_dtype, const void* inp, int in_dtype, const i
         ScratchNeed need;
         gemm_tc_scratch_need(a, d.num_sms, &need.ws, &need.counters);
         TcScratch scratch;
-        if ((st = get_scratch(need, d.num_sms, stream, &scratch))) return st;
+        if ((st = get_scratch(need, d.num_sms, stream, &hold, &scratch))) return st;
         e = launch_q8_gemm_tc(a, d.num_sms, scratch, stream);
         if (e != cudaSuccess) return cuda_fail(e, "q8_gemm_tc launch");
         return B200Q8_OK;
@@ -421,7 +406,7 @@ int linear_impl(void* out, int out_dtype, const void* inp, int in_dtype, const i
             ScratchNeed need;
             gemv_i8_scratch_need(b, d.num_sms, &need.ws, &need.counters, &need.act, &need.exps);
             TcScratch scratch;
-            if ((st = get_scratch(need, d.num_sms, stream, &scratch))) return st;
+            if ((st = get_scratch(need, d.num_sms, stream, &hold, &scratch))) return st;
             e = launch_q8_gemv_i8(b, d.num_sms, scratch, stream);
             if (e != cudaSuccess) return cuda_fail(e, "q8_gemv_i8 launch");
         }
@@ -450,22 +435,26 @@ int linear_impl(void* out, int out_dtype, const void* inp, int in_dtype, const i
 
 }  // namespace
 
-int stream_scratch(size_t ws_floats, size_t counters, size_t act_bytes, int num_sms, cudaStream_t stream, TcScratch* out)
+int stream_scratch(size_t ws_floats, size_t counters, size_t act_bytes, int num_sms, cudaStream_t stream, ScratchHold* hold,
+                   TcScratch* out)
 {
     ScratchNeed need;
     need.ws = ws_floats;
     need.counters = counters;
     need.act = act_bytes;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+    const StreamKey key = stream_key(dev, stream, cudaStreamPerThread);
+    g_scratch.hold(key, hold);  // (threads that capture on one stream take turns too)
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
     unsigned long long capture = 0;
     cudaGraph_t graph = nullptr;
-    cudaError_t e = cudaStreamGetCaptureInfo_v2(stream, &status, &capture, &graph, nullptr, nullptr);
+    e = cudaStreamGetCaptureInfo_v2(stream, &status, &capture, &graph, nullptr, nullptr);
     if (e != cudaSuccess) return cuda_fail(e, "cudaStreamGetCaptureInfo");
-    if (status == cudaStreamCaptureStatusNone) return get_scratch(need, num_sms, stream, out);
+    if (status == cudaStreamCaptureStatusNone) return get_scratch(need, num_sms, stream, hold, out);
     if (status != cudaStreamCaptureStatusActive) return cuda_fail(cudaErrorStreamCaptureInvalidated, "stream capture");
-    int dev = 0;
-    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-    return capture_scratch(need, dev, stream, capture, graph, out);
+    return capture_scratch(need, key, capture, graph, out);
 }
 
 int current_device(int* num_sms, size_t* max_smem)
@@ -611,6 +600,8 @@ int b200q8_linear_q8_noalloc(void* out, int out_dtype, const void* inp, int in_d
     a.out_dtype = out_dtype;
     a.pdl = true;
     cudaError_t e = cudaSuccess;
+    static std::mutex& order = *new std::mutex;  // a call's clearing and kernels, on the one array, stay together
+    std::lock_guard<std::mutex> lk(order);
     switch (launch_q8_gemv_i8_noalloc(a, d.num_sms, (cudaStream_t)stream, &e)) {
         case 0: return B200Q8_OK;
         case 1: return fail(B200Q8_ERR_UNSUPPORTED, "linear_q8_noalloc: M=%zu exceeds the fixed scratch (at most 2 tokens)", M);
@@ -680,8 +671,9 @@ int b200q8_diag_peer_wait(const uint64_t* counts, int n, int self, double timeou
         return fail(B200Q8_ERR_UNSUPPORTED, "diag_peer_wait: K=%zu is scanned by the prep kernel (use where=2)", K);
     ScratchNeed need;
     gemv_i8_scratch_need(a, d.num_sms, &need.ws, &need.counters, &need.act, &need.exps);
+    ScratchHold hold;
     TcScratch scratch;
-    if ((st = get_scratch(need, d.num_sms, (cudaStream_t)stream, &scratch))) return st;
+    if ((st = get_scratch(need, d.num_sms, (cudaStream_t)stream, &hold, &scratch))) return st;
     e = launch_q8_gemv_i8(a, d.num_sms, scratch, (cudaStream_t)stream);
     return e == cudaSuccess ? B200Q8_OK : cuda_fail(e, "diag_peer_wait: GEMV launch");
 }
@@ -727,8 +719,9 @@ int b200q8_linear_q8_argmax(void* out, int out_dtype, const void* inp, int in_dt
     ScratchNeed need;
     gemv_i8_scratch_need(a, d.num_sms, &need.ws, &need.counters, &need.act, &need.exps);
     need.amax = true;
+    ScratchHold hold;
     TcScratch scratch;
-    if ((st = get_scratch(need, d.num_sms, (cudaStream_t)stream, &scratch))) return st;
+    if ((st = get_scratch(need, d.num_sms, (cudaStream_t)stream, &hold, &scratch))) return st;
     a.amax_keys = scratch.amax;
     a.amax_done = reinterpret_cast<unsigned int*>(scratch.amax + kMaxArgmaxTokens);
     a.amax_out = argmax;
@@ -1477,8 +1470,9 @@ int b200q8_linear_q8_sharded_p2p_ex(b200q8_comm* c, void* out, int out_dtype, co
                                             "aligned pointers (K=%zu)", K);
     ScratchNeed need;
     gemv_i8_scratch_need(a, d.num_sms, &need.ws, &need.counters, &need.act, &need.exps);
+    ScratchHold hold;
     TcScratch scratch;
-    if ((st = get_scratch(need, d.num_sms, (cudaStream_t)stream, &scratch))) return st;
+    if ((st = get_scratch(need, d.num_sms, (cudaStream_t)stream, &hold, &scratch))) return st;
     // A deferred wait of the previous call is owed before this call reads its input: it is paid
     // inside whichever of this call's kernels reads x first (the GEMV, or its prep kernel).
     if (c->pending) {

@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "stream_order.h"
+
 namespace b200q8 {
 
 enum DType : int { kF32 = 0, kF16 = 1 };
@@ -227,8 +229,11 @@ cudaError_t launch_prologue(int pro, const void* x, void* out, int dtype, const 
                             size_t K, bool pdl, cudaStream_t stream);
 
 // Scratch of the sizes given for a call on the stream: that of (current device, stream), or, during a capture, the
-// captured graph's own; a status.
-int stream_scratch(size_t ws_floats, size_t counters, size_t act_bytes, int num_sms, cudaStream_t stream, TcScratch* out);
+// captured graph's own; a status.  `hold` is to live until the call's last launch: until then no other host
+// thread's call on the stream queues launches that use it.
+using ScratchHold = PerStream<TcScratch>::Held;
+int stream_scratch(size_t ws_floats, size_t counters, size_t act_bytes, int num_sms, cudaStream_t stream, ScratchHold* hold,
+                   TcScratch* out);
 
 // SM count and opt-in shared memory of the current device, as a status (B200Q8_ERR_UNSUPPORTED: not sm_100).
 int current_device(int* num_sms, size_t* max_smem);

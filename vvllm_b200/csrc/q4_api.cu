@@ -115,12 +115,13 @@ int linear_q4(const char* what, void* out, int out_dtype, const void* inp, int i
     Q4Args fast = a;  // as it will be after the copying
     if (pad) fast.q4 = nullptr, fast.x = nullptr, fast.K = (K + 31) / 32 * 32;
     const bool use_gemm = gemm && q4_gemm_tc_supports(fast);
+    ScratchHold hold;  // to the last launch below
     if (use_gemm || pad) {
         size_t ws = 0, counters = 0, act = 0;
         if (use_gemm) q4_gemm_tc_scratch_need(fast, sms, &ws, &counters, &act);
         act = (act + 255) / 256 * 256;
         TcScratch scratch;
-        if ((st = stream_scratch(ws, counters, act + pad, sms, stream, &scratch))) return st;
+        if ((st = stream_scratch(ws, counters, act + pad, sms, stream, &hold, &scratch))) return st;
         cudaError_t e = pad ? launch_q4_pad(&a, scratch.act + act, sms, stream) : cudaSuccess;
         if (e != cudaSuccess) return cuda_fail(e, "q4_pad launch");
         if (use_gemm) {
