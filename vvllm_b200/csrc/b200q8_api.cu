@@ -103,24 +103,51 @@ struct ScratchNeed {
     bool amax = false;
 };
 
-// Grows one device buffer of `s` to at least `need` elements (never shrinks).  The buffer it replaces is kept
-// until exit: a graph captured earlier may still hold it.  Sizes at least double, so those kept add up to
-// less than the one in use.
+// Buffers up to this size at least double where they grow (a graph's are rounded up to a power of two), so that a
+// slowly growing need is met in few allocations; larger ones, which may be copies of whole matrices, take
+// what is needed.
+constexpr size_t kRoundedBytes = (size_t)64 << 20;
+
+size_t free_idle_capture_scratch(int dev);
+
+// Grows one device buffer of `s` to at least `need` elements, `dflt` if there is room (never shrinks).  With `keep` a
+// graph captured earlier may still hold the buffer it replaces, which then stays until exit; sizes double as long as
+// there is room, so that those kept add up to less than the one in use.
 template <typename T>
-int grow(T** buf, size_t* have, size_t need, size_t dflt, cudaStream_t stream, bool zero, const char* what)
+int grow(T** buf, size_t* have, size_t need, size_t dflt, int dev, cudaStream_t stream, bool zero, bool keep, const char* what)
 {
     if (*have >= need) return B200Q8_OK;
     size_t n = need > dflt ? need : dflt;
-    if (n < 2 * *have) n = 2 * *have;
+    if (n < 2 * *have && (keep || 2 * *have * sizeof(T) <= kRoundedBytes)) n = 2 * *have;
     T* nb = nullptr;
-    cudaError_t e = cudaMalloc(&nb, n * sizeof(T));
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        return fail(B200Q8_ERR_ALLOC, "scratch %s: cudaMalloc(%zu): %s", what, n * sizeof(T), cudaGetErrorString(e));
+    auto alloc = [&](size_t count) {
+        n = count;
+        const cudaError_t r = cudaMalloc(&nb, n * sizeof(T));
+        if (r != cudaSuccess) cudaGetLastError();
+        return r;
+    };
+    auto drop = [&]() -> cudaError_t {  // queued work on the stream may still use the old buffer
+        if (!*buf || keep) return cudaSuccess;
+        cudaError_t r = cudaStreamSynchronize(stream);
+        if (r == cudaSuccess) r = cudaFree(*buf);
+        *buf = nullptr;
+        *have = 0;
+        return r;
+    };
+    cudaError_t e = alloc(n);
+    if (e == cudaErrorMemoryAllocation && n > need) e = alloc(need);
+    if (e == cudaErrorMemoryAllocation && free_idle_capture_scratch(dev)) e = alloc(need);
+    if (e == cudaErrorMemoryAllocation && *buf && !keep) {
+        if ((e = drop()) != cudaSuccess) return cuda_fail(e, "scratch release");
+        e = alloc(need);
     }
-    if (zero && (e = cudaMemsetAsync(nb, 0, n * sizeof(T), stream)) != cudaSuccess) {
+    if (e != cudaSuccess)
+        return fail(B200Q8_ERR_ALLOC, "scratch %s: cudaMalloc(%zu): %s", what, n * sizeof(T), cudaGetErrorString(e));
+    if (zero) e = cudaMemsetAsync(nb, 0, n * sizeof(T), stream);
+    if (e == cudaSuccess) e = drop();
+    if (e != cudaSuccess) {
         cudaFree(nb);
-        return cuda_fail(e, "scratch memset");
+        return cuda_fail(e, "scratch memset or release");
     }
     *buf = nb;
     *have = n;
@@ -135,16 +162,23 @@ int get_scratch(const ScratchNeed& need, int num_sms, cudaStream_t stream, Scrat
     if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
     g_scratch.hold(stream_key(dev, stream, cudaStreamPerThread), hold);
     TcScratch& s = **hold;
+    // From its first captured call on, a graph may hold the stream's buffers (where the status cannot be told, too).
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (!s.in_graph && (cudaStreamIsCapturing(stream, &status) != cudaSuccess || status != cudaStreamCaptureStatusNone)) {
+        cudaGetLastError();
+        s.in_graph = true;
+    }
+    const bool keep = s.in_graph;
     // Default capacities: 128-column partials on every SM, 64K tiles.
     int st;
-    if ((st = grow(&s.ws, &s.ws_floats, need.ws, (size_t)2 * num_sms * 128 * 128, stream, false, "partials")) ||
-        (st = grow(&s.counter_ptr, &s.counters, need.counters, (size_t)1 << 16, stream, true, "counters")) ||
-        (st = grow(&s.exps, &s.exps_count, need.exps, (size_t)320, stream, false, "exponent words")) ||
-        (st = grow(&s.act, &s.act_bytes, need.act, 0, stream, false, "prologue activations")))
+    if ((st = grow(&s.ws, &s.ws_floats, need.ws, (size_t)2 * num_sms * 128 * 128, dev, stream, false, keep, "partials")) ||
+        (st = grow(&s.counter_ptr, &s.counters, need.counters, (size_t)1 << 16, dev, stream, true, keep, "counters")) ||
+        (st = grow(&s.exps, &s.exps_count, need.exps, (size_t)320, dev, stream, false, keep, "exponent words")) ||
+        (st = grow(&s.act, &s.act_bytes, need.act, 0, dev, stream, false, keep, "prologue activations")))
         return st;
     if (need.amax && !s.amax) {  // argmax keys + done counter, zero at rest
         size_t have = 0;
-        if ((st = grow(&s.amax, &have, (size_t)kMaxArgmaxTokens + 1, 0, stream, true, "argmax")))
+        if ((st = grow(&s.amax, &have, (size_t)kMaxArgmaxTokens + 1, 0, dev, stream, true, keep, "argmax")))
             return st;
     }
     *out = s;
@@ -153,8 +187,9 @@ int get_scratch(const ScratchNeed& need, int num_sms, cudaStream_t stream, Scrat
 
 // Scratch of calls captured into a graph: the graph's own, so that its replays may run beside other calls
 // on the stream of the capture and beside other graphs.  One set per (capture, stream), held by the
-// graph (and what is instantiated from it) through a user object; when the last of them is destroyed the
-// set goes back to be taken by a later capture.  Never destroyed, as graphs may outlive this library's statics.
+// graph (and what is instantiated from it: those share it) through a user object; when the last of them is
+// destroyed the set is idle, to be taken by a later capture or freed where a later call needs memory
+// that it does not fit.  The list is never destroyed, as graphs may outlive this library's statics.
 struct CaptureScratch {
     bool taken = false;
     unsigned long long capture = 0;  // whose calls on `stream` it serves
@@ -170,54 +205,98 @@ void CUDART_CB release_capture_scratch(void* p)  // may not call CUDA
     static_cast<CaptureScratch*>(p)->taken = false;
 }
 
+size_t capture_bytes(size_t ws, size_t counters, size_t act) { return ws * sizeof(float) + counters * sizeof(int) + act; }
+
 bool holds(const TcScratch& s, const ScratchNeed& need)
 {
     return s.ws_floats >= need.ws && s.counters >= need.counters && s.act_bytes >= need.act;
 }
 
+void free_buffers(TcScratch* s)
+{
+    cudaFree(s->ws);
+    cudaFree(s->counter_ptr);
+    cudaFree(s->act);
+    cudaGetLastError();
+    *s = TcScratch{};
+}
+
+// Frees the sets of a device that no graph holds any more; how many bytes.  Not for a thread whose capture
+// forbids it (fill_capture_scratch lifts that).
+size_t free_idle_capture_scratch(int dev)
+{
+    std::vector<CaptureScratch*> idle;
+    {
+        std::lock_guard<std::mutex> lk(g_capture_mu);
+        size_t kept = 0;
+        for (CaptureScratch* c : g_capture) {
+            if (c->taken || c->stream.dev != dev)
+                g_capture[kept++] = c;
+            else
+                idle.push_back(c);
+        }
+        g_capture.resize(kept);
+    }
+    size_t bytes = 0;
+    for (CaptureScratch* c : idle) {
+        bytes += capture_bytes(c->s.ws_floats, c->s.counters, c->s.act_bytes);
+        free_buffers(&c->s);
+        delete c;
+    }
+    return bytes;
+}
+
 // Allocates during a capture, which goes on: this thread's calls are let through, and the counters are
 // zeroed on a stream of their own.
-int fill_capture_scratch(const ScratchNeed& need, bool fresh, TcScratch* s)
+int fill_capture_scratch(const ScratchNeed& need, bool fresh, int dev, TcScratch* s)
 {
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
     cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
     if (e != cudaSuccess) return cuda_fail(e, "cudaThreadExchangeStreamCaptureMode");
     cudaStream_t own = nullptr;
     int st = B200Q8_OK;
+    if (fresh) free_idle_capture_scratch(dev);  // none of them fits
     if ((e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking)) != cudaSuccess) st = cuda_fail(e, "cudaStreamCreate");
-    if (!st && fresh &&
-        ((st = grow(&s->ws, &s->ws_floats, need.ws, 0, own, false, "partials")) ||
-         (st = grow(&s->counter_ptr, &s->counters, need.counters, (size_t)1 << 12, own, false, "counters")) ||
-         (st = grow(&s->act, &s->act_bytes, need.act, 0, own, false, "scales")))) {
-        cudaFree(s->ws);
-        cudaFree(s->counter_ptr);
-    }
+    if (!st && fresh) st = grow(&s->ws, &s->ws_floats, need.ws, 0, dev, own, false, true, "partials");
+    if (!st && fresh) st = grow(&s->counter_ptr, &s->counters, need.counters, (size_t)1 << 12, dev, own, false, true, "counters");
+    if (!st && fresh) st = grow(&s->act, &s->act_bytes, need.act, 0, dev, own, false, true, "scales");
     if (!st && (e = cudaMemsetAsync(s->counter_ptr, 0, s->counters * sizeof(int), own)) != cudaSuccess)
         st = cuda_fail(e, "scratch memset");
     if (!st && (e = cudaStreamSynchronize(own)) != cudaSuccess) st = cuda_fail(e, "scratch memset");
     if (own) cudaStreamDestroy(own);
+    if (st && fresh) free_buffers(s);
     cudaThreadExchangeStreamCaptureMode(&mode);
     return st;
 }
 
 int capture_scratch(ScratchNeed need, const StreamKey& stream, unsigned long long capture, cudaGraph_t graph, TcScratch* out)
 {
-    // In powers of two, so that a later capture finds one that fits.
-    for (size_t* n : {&need.ws, &need.counters, &need.act}) {
+    // Rounded, so that a later capture finds one that fits.
+    const struct {
+        size_t* n;
+        size_t size;
+    } parts[] = {{&need.ws, sizeof(float)}, {&need.counters, sizeof(int)}, {&need.act, 1}};
+    for (const auto& p : parts) {
         size_t up = 1024;
-        while (up < *n) up *= 2;
-        *n = up;
+        if (*p.n * p.size <= kRoundedBytes)
+            while (up < *p.n) up *= 2;
+        else
+            up = (*p.n + 4095) / 4096 * 4096;
+        *p.n = up;
     }
+    const size_t most = 2 * capture_bytes(need.ws, need.counters, need.act) + kRoundedBytes;
     CaptureScratch* c = nullptr;
     {
         std::lock_guard<std::mutex> lk(g_capture_mu);
+        size_t least = most + 1;
         for (CaptureScratch* i : g_capture) {
             if (i->stream.dev != stream.dev || !holds(i->s, need)) continue;
             if (i->taken && i->capture == capture && i->stream == stream) {
                 *out = i->s;
                 return B200Q8_OK;
             }
-            if (!i->taken && (!c || i->s.ws_floats < c->s.ws_floats)) c = i;
+            const size_t bytes = capture_bytes(i->s.ws_floats, i->s.counters, i->s.act_bytes);
+            if (!i->taken && bytes < least) c = i, least = bytes;
         }
         if (c) {
             c->taken = true;
@@ -232,7 +311,7 @@ int capture_scratch(ScratchNeed need, const StreamKey& stream, unsigned long lon
         c->capture = capture;
         c->stream = stream;
     }
-    const int st = fill_capture_scratch(need, fresh, &c->s);
+    const int st = fill_capture_scratch(need, fresh, stream.dev, &c->s);
     if (st) {
         if (fresh)
             delete c;

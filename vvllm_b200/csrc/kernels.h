@@ -125,6 +125,7 @@ struct TcScratch {
     unsigned char* act = nullptr;  // activations a prologue wrote for the following GEMV / GEMM
     size_t act_bytes = 0;
     unsigned long long* amax = nullptr;  // argmax keys [kMaxArgmaxTokens] + a counter word, zero at rest
+    bool in_graph = false;  // a captured graph may hold these buffers
 };
 constexpr int kMaxArgmaxTokens = 64;
 
