@@ -285,7 +285,9 @@ B200Q8_API int b200q8_dequantize_q4(void* out, int out_dtype, const uint8_t* q4,
  * These and fp16 calls of more than 8 tokens share a scratch per stream, allocated (cudaMalloc) with the first
  * such call and kept at the size of the largest so far: partial sums and scales (some 20 to 60 MB), and the copied rows (as
  * much as the matrix).  Captured into a graph they get scratch of the graph's own, of that size again for each
- * graph, also where it is the stream's first call: graphs may be replayed on any streams, beside each other. */
+ * graph, also where it is the stream's first call: graphs may be replayed on any streams, beside each other.
+ * What is instantiated from one captured graph or its clones shares that graph's scratch, and must not run at the
+ * same time: capture once for each executable that is to. */
 B200Q8_API int b200q8_linear_q4(void* out, int out_dtype, const void* inp, int in_dtype, const uint8_t* q4,
                                 const uint16_t* scales, int group, const float* bias, size_t M, size_t N, size_t K,
                                 b200q8_stream_t stream);
