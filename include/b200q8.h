@@ -275,10 +275,15 @@ B200Q8_API int b200q8_dequantize_q4(void* out, int out_dtype, const uint8_t* q4,
                                     const int32_t* rows, size_t R, size_t N, size_t K, b200q8_stream_t stream);
 
 /* out[M, N] = inp[M, K] . w[N, K]^T + bias[N]; bias may be NULL.  inp and out are fp32 or fp16; any M.
- * Weights are used as they are, q * s with all its bits, and sums are fp32, whatever the types.  What is rounded
- * before them: with fp32 inputs, and fp16 at one or two tokens, an input, by at most 2^-22 of the
- * largest |inp| of its 128 consecutive ones, or 2^-123; with fp16 inputs and more than 8 tokens, a scale
- * below 2^-29 of its row's largest.  Scales' magnitudes are to be below 2^90.
+ * Weights are used as they are, q * s with all its bits, and sums are fp32, whatever the types (many tokens with
+ * fp16 outputs: the tensor core's, which cut instead of rounding, less than a tenth of an fp16 step over
+ * 18944 products).  What is rounded before them: with fp32 inputs, and fp16 at one or two tokens, an input, by at
+ * most 2^-22 of the largest |inp| of its 128 consecutive ones, or 2^-123 (so beside an activation of 1000
+ * the others are held in steps of 2.4e-4); with fp16 inputs and more than 8 tokens, a scale below 2^-29 of its
+ * row's largest.  Scales' magnitudes are to be below 2^90.
+ * One or two tokens, more of them, and many take kernels that sum in different orders and round as above: the same
+ * token's outputs may differ in their last bits with the number of tokens beside it.  Calls of the same
+ * sizes, types and alignment on the same GPU give the same bits every time.
  * An infinity or NaN in inp reaches its own row of out only, as the formula has it.
  * K a multiple of 32 with inp and q4 16-byte aligned is read as it lies; else larger calls first copy
  * the weights and tokens into such rows, in scratch of their size.
