@@ -337,7 +337,8 @@ typedef struct b200q8_logit_rules {
  *   out[m, i] = v in out_dtype;  argmax[m] = the first largest out[m, i] among the allowed i, in the
  *   order of b200q8_linear_q8_argmax (a NaN wins only as the first allowed token); -1 if none is allowed.
  * out may be NULL (only the tokens are wanted), or logits itself (same type and stride); it must not
- * overlap logits otherwise.  argmax (int32 [M]) may be NULL.  rules may be NULL.  Token ids outside
+ * overlap logits otherwise.  argmax (int32 [M]) may be NULL.  rules may be NULL.  Biases come behind the penalties:
+ * where a server adds them first, a token that is both biased and in the history gets another value there.  Token ids outside
  * [0, V) in the lists are ignored; lengths are clamped to [0, history_count] and [0, bias_count].
  * Each operation is IEEE's, also where a penalty is 0, negative, infinite or NaN.  One launch, no scratch. */
 B200Q8_API int b200q8_process_logits(void* out, int out_dtype, size_t out_stride, const void* logits, int in_dtype,

@@ -461,7 +461,8 @@ def process_logits(out, logits, argmax=None, history=None, history_len=None, pro
 
     out: fp32 or fp16, logits itself, or None.  history / bias_ids / bias_values / allowed: [M, n]
     int32 / int32 / fp32 / int32 (bit i % 32 of word i // 32), or one row for all; the other rules are
-    [M]: int32 lengths and fp32 penalties.  Rows of every 2-D tensor are contiguous, any row stride."""
+    [M]: int32 lengths and fp32 penalties.  Rows of every 2-D tensor are contiguous, any row stride.
+    The penalties come first, then the biases, then the mask."""
     name, T = "process_logits", _torch or _t()
     M, V = logits.shape
     i32, f32, per = T.int32, T.float32, (M,)

@@ -96,9 +96,11 @@ int linear_q4(const char* what, void* out, int out_dtype, const void* inp, int i
     a.in_dtype = in_dtype;
     a.out_dtype = out_dtype;
     // The streaming kernel goes over the weights once for every 16 fp16 tokens (8 in fp32), in passes that run side by
-    // side; the GEMM (fp16 tokens) once, at a rate bound by its dequantization and with a start of its own.
+    // side; the GEMM (fp16 tokens) once, bound by its dequantization at 64 tokens and with a start of its own.
     // Measured on B200, streaming vs GEMM: 37888 x 3584 at 16 tokens 24 vs 38 us, at 17 39 vs 38; 3584 x 3584 at 64 16
     // vs 21, at 128 25 vs 24; 896 x 4864 at 64 12 vs 26, at 256 26 vs 25; 4864 x 896 at 32 9 vs 10, at 64 11 vs 10.
+    // With K of a few hundred the rule takes the GEMM too early: 37888 x 256 at 32 9 vs 13, x 512 11 vs 14; 9600 x 256 at
+    // 300 16 vs 23, x 128 18 vs 22.
     // Up to 16 tokens only those that need clusters of eight are slower: 3584 x 18944 at 9 24 vs 28, at 16 38 vs 28;
     // 8192 x 28672 at 8 38 vs 64, at 9 72 vs 64.
     const size_t work = M * N * K;

@@ -108,8 +108,10 @@ cudaError_t launch_generic(const Q4Args& a, cudaStream_t stream)
 // weights) to 16 tokens.
 //
 // Bound by HBM (half a byte a weight) for one and two tokens once there are megabytes to stream: 152064 x 3584
-// at 46 us, 6.1 TB/s; 37888 x 3584 at 13.4 us, of which 3 are start and tokens.  With more, by instruction issue
-// and its dependences: 8 tokens, 152064 x 3584 64 us, 37888 x 3584 17; 16 tokens 93 and 24.5; with long K also by
+// at 46 us, 6.1 TB/s; 37888 x 3584 at 13.4 us, of which 3 are start and tokens.  With more, by latencies: at 8 tokens no
+// unit is full (issue slots 59 %, ALU 50 %, tensor pipe 23 %), and 16 warps an SM do not cover the chain from a
+// box over its unpacking to its products: 8 tokens, 152064 x 3584 64 us, 37888 x 3584 17; 16 tokens 93 and 24.5; three
+// and eight fp32 ones 24 and 26.5 (three products a token's byte); with long K also by
 // the tokens' way into shared memory: 3584 x 18944 12 us at one, 17.5 at eight.
 //
 // Work: a tile is 16 rows; an item is a tile's next 256 or 512 of K.  `wk` warps share a tile (item ch
@@ -201,7 +203,8 @@ __device__ __forceinline__ void mma16832(int (&d)[4], int start, uint32_t a0, ui
 }
 
 // The eight codes of a word as the integers q in fp16: elements (0, 4), (1, 5), (2, 6), (3, 7).  A code in the low
-// bits of 1024.0 is 1024 + code, one four bits up 1024 + 16 code; one packed fma leaves q.
+// bits of 1024.0 is 1024 + code, one four bits up 1024 + 16 code; one packed fma leaves q.  (Converting small integers
+// under an exponent: Kim, Henry, Fahim and Awadalla, "Who Says Elephants Can't Run", 2022.)
 __device__ __forceinline__ void unpack8_halves(uint32_t w, uint32_t (&h)[4])
 {
 #pragma unroll

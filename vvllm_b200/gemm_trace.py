@@ -4,6 +4,7 @@
     python -m vvllm_b200.gemm_trace phases [KxN ...]   # per-CTA phase times of one launch after an L2 flush
     python -m vvllm_b200.gemm_trace sweep              # per-call time back to back, every tile width / grid
     python -m vvllm_b200.gemm_trace roles KxN:M ...    # per-role wait / loop cycles per K-stage of one launch
+                                                       # (KxN:M:4 on 4-bit weights, group 128)
 
 The profiling copy is the same sources built with -DB200Q8_TRACE: the GEMM then stamps each CTA's
 phases (%globaltimer at its start, SM cycles to each phase after it) into a device array that
@@ -120,26 +121,34 @@ def roles(cases) -> None:
     L.b200q8_trace_gemm_roles.restype = ctypes.c_int
     dev = torch.device("cuda", 0)
     for case in cases:
-        shape, _, m = case.partition(":")
+        shape, m, bits = (case.split(":") + ["", ""])[:3]
         K, N = (int(a) for a in shape.split("x"))
-        Mt = int(m or M)
-        q = torch.randint(-127, 128, (N, K), dtype=torch.int8, device=dev)
-        s = torch.rand(N, device=dev) * 1e-3
+        Mt, bits = int(m or M), int(bits or 8)
         x = torch.randn(Mt, K, device=dev).half()
         out = torch.empty(Mt, N, device=dev, dtype=torch.float16)
+        if bits == 8:
+            q = torch.randint(-127, 128, (N, K), dtype=torch.int8, device=dev)
+            s = torch.rand(N, device=dev) * 1e-3
+        else:
+            q = torch.randint(0, 256, (N, K // 2), dtype=torch.uint8, device=dev)
+            s = (0.01 + 0.01 * torch.rand(N, K // 128, device=dev)).bfloat16()
+
+        def call():
+            v.linear_q8(out, x, q, s) if bits == 8 else v.linear_q4(out, x, q, s, 128)
+
         for _ in range(3):
-            v.linear_q8(out, x, q, s)
+            call()
         torch.cuda.synchronize()
         buf = np.zeros((1024, 16), dtype=np.uint64)
         L.b200q8_trace_gemm_roles(None, 0)  # cleared: CTAs of earlier launches leave no counts
         torch.cuda.synchronize()
-        v.linear_q8(out, x, q, s)
+        call()
         torch.cuda.synchronize()
         L.b200q8_trace_gemm_roles(buf.ctypes.data, buf.nbytes)
         live = buf[:, 3] > 0
         st = np.maximum(buf[live, 4].astype(np.float64), 1.0)
         per = {name: round(float(np.median(buf[live, i] / st)), 1) for i, name in enumerate(ROLE_SLOTS) if i != 4}
-        print(f"K={K} N={N} M={Mt}", json.dumps(dict(ctas=int(live.sum()), stages_median=float(np.median(st)),
+        print(f"K={K} N={N} M={Mt} {bits} bit", json.dumps(dict(ctas=int(live.sum()), stages_median=float(np.median(st)),
                                                    loop_us=round(float(np.median(buf[live, 3])) / SM_MHZ, 2),
                                                    cycles_per_stage=per)), flush=True)
 
