@@ -169,3 +169,39 @@ def test_threads_that_capture_and_call(cuda):
     assert not errors, errors
     for (_, want), out in zip(jobs, outs):
         assert np.array_equal(out.cpu().numpy(), want.cpu().numpy())
+
+
+FIRST_CALLS = """
+import threading
+import torch
+import vvllm_b200 as v
+
+x, q4 = torch.ones((24, 64), device="cuda").half(), torch.full((300, 32), 0x99, dtype=torch.uint8, device="cuda")
+sc = torch.ones((300, 1), dtype=torch.bfloat16, device="cuda")
+outs = [torch.zeros((24, 300), device="cuda") for _ in range(16)]
+torch.cuda.synchronize()
+v.lib()
+gate = threading.Barrier(16)
+
+def work(o):
+    gate.wait()
+    v.linear_q4(o, x, q4, sc, 64)
+
+threads = [threading.Thread(target=work, args=(o,)) for o in outs]
+[t.start() for t in threads]
+[t.join() for t in threads]
+torch.cuda.synchronize()
+assert all((o == 64).all() for o in outs)
+print("ok")
+"""
+
+
+def test_the_first_calls_of_a_process_at_once(cuda):
+    """What the library looks up once a process is looked up by sixteen threads together."""
+    import subprocess
+    import sys
+
+    from tests.conftest import ROOT
+
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr

@@ -53,11 +53,11 @@ struct DeviceInfo {
     int num_sms = 0;
     size_t max_smem = 0;  // opt-in dynamic shared memory per block
     int cc_major = 0, cc_minor = 0;
-    bool valid = false;
 };
 
 constexpr int kMaxDevices = 64;
 DeviceInfo g_dev[kMaxDevices];
+std::atomic<bool> g_dev_known[kMaxDevices];  // set, for good, once the entry is written
 std::mutex g_dev_mu;
 
 int device_info(DeviceInfo* out)
@@ -66,9 +66,9 @@ int device_info(DeviceInfo* out)
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
     if (dev < 0 || dev >= kMaxDevices) return fail(B200Q8_ERR_UNSUPPORTED, "device %d out of range", dev);
-    if (!g_dev[dev].valid) {
+    if (!g_dev_known[dev].load(std::memory_order_acquire)) {
         std::lock_guard<std::mutex> lk(g_dev_mu);
-        if (!g_dev[dev].valid) {
+        if (!g_dev_known[dev].load(std::memory_order_relaxed)) {
             DeviceInfo d;
             int v = 0;
             if ((e = cudaDeviceGetAttribute(&d.num_sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess)
@@ -78,8 +78,8 @@ int device_info(DeviceInfo* out)
             d.max_smem = (size_t)v;
             cudaDeviceGetAttribute(&d.cc_major, cudaDevAttrComputeCapabilityMajor, dev);
             cudaDeviceGetAttribute(&d.cc_minor, cudaDevAttrComputeCapabilityMinor, dev);
-            d.valid = true;
             g_dev[dev] = d;
+            g_dev_known[dev].store(true, std::memory_order_release);
         }
     }
     *out = g_dev[dev];
